@@ -1,0 +1,372 @@
+// Backward pass of the residual norm (residual_norm_fwd.hip).  With h = post(f), fhat and rhat the
+// normalised branch and stream rows, s1 and s2 their 1/std, a the residual and b the branch scale:
+//
+//   t  = dy * w_pre                       dw_pre = sum_rows dy * rhat        db_pre = sum_rows dy
+//   g  = dr + s2 * (t - mean(t) - rhat * mean(t * rhat))                     the gradient of r
+//   dx = a * g                            dgate  = b * g * h, summed over what the gate is shared by
+//   d  = b * gate * g                     dw_post = sum_rows d * fhat        db_post = sum_rows d
+//   u  = d * w_post                       df = s1 * (u - mean(u) - fhat * mean(u * fhat))
+//
+// (an rms norm has no mean(t), mean(u)).  r is formed again from x and f: what the forward pass
+// normalised was r before it was rounded to its type, and x and f are read for the rest anyway.
+//
+// Bound: memory.  One pass reads x, f, dr, dy (and an element-wise gate) and writes dx, df (and its
+// gradient).  The sums over rows stay in registers while a team walks its rows, four per column:
+// sum dy * rhat, sum dy, sum c * g * fhat, sum c * g with c the gate of the row or element, 1 for a
+// channel gate -- that one is the same for every row and is multiplied in at the end, and
+// dgate = b * (w_post * sum g * fhat + b_post * sum g) needs no sum of its own.  Teams of a block meet
+// in registers and LDS, blocks leave one partial row each, a second kernel adds the partial rows in
+// block order: no atomics, and the grid depends on the shape alone, so results repeat bit for bit.
+#include "residual_norm.hpp"
+
+namespace cxg {
+namespace {
+
+constexpr int kRnMaxBlocks = 1024;       // partial rows
+
+template <typename TX, typename TF, int V, int L, int ITEMS>
+__global__ __launch_bounds__(kRnThreads) void residual_norm_bwd_kernel(RnArgs a) {
+  __shared__ float s_red[2][kRnThreads / CXG_WAVE][2];
+  constexpr int kTeams = kRnThreads / L;
+  const int lit = threadIdx.x % L, team = threadIdx.x / L;
+  const int cols = a.cols;
+  const float inv_c = 1.0f / (float)cols;
+  int slot = 0;
+  const bool post = a.post_kind != CXG_NORM_NONE, pre = a.pre_kind != CXG_NORM_NONE;
+  const bool post_layer = a.post_kind == CXG_NORM_LAYER, pre_layer = a.pre_kind == CXG_NORM_LAYER;
+  float w1[ITEMS][V], b1[ITEMS][V], w2[ITEMS][V], gc[ITEMS][V];
+  // columns that do not exist have weight 0 and so add nothing to the sums over a row
+  rn_params<L, V, ITEMS>(post ? a.post_w : nullptr, cols, lit, 1.f, w1);
+  rn_params<L, V, ITEMS>(post ? a.post_b : nullptr, cols, lit, 0.f, b1);
+  rn_params<L, V, ITEMS>(pre ? a.pre_w : nullptr, cols, lit, 1.f, w2);
+  rn_params<L, V, ITEMS>(a.gate_kind == CXG_GATE_CHANNEL ? static_cast<const float*>(a.gate) : nullptr, cols, lit, 1.f, gc);
+  bool in[ITEMS];
+  float sums[kRnSums][ITEMS][V];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    in[i] = rn_col<L, V>(i, lit) < cols;
+#pragma unroll
+    for (int q = 0; q < kRnSums; ++q)
+#pragma unroll
+      for (int j = 0; j < V; ++j) sums[q][i][j] = 0.f;
+  }
+
+  for (int64_t base = (int64_t)blockIdx.x * kTeams; base < a.rows; base += (int64_t)gridDim.x * kTeams) {
+    const int64_t row = base + team;
+    const bool live = row < a.rows;
+    const int64_t rr = live ? row : 0;
+    Piece<TX, V> px[ITEMS], pdr[ITEMS];
+    Piece<TF, V> pf[ITEMS], pg[ITEMS], pdy[ITEMS];
+    const TX* const xrow = static_cast<const TX*>(a.x) + rr * a.ldx;
+    const TF* const frow = static_cast<const TF*>(a.f) + rr * a.ldf;
+    const TX* const drrow = static_cast<const TX*>(a.dr) + rr * a.lddr;
+    const TF* const dyrow = static_cast<const TF*>(a.dy) + rr * a.lddy;
+    const bool full = a.gate_kind == CXG_GATE_FULL;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      px[i].clear(); pf[i].clear(); pdr[i].clear(); pdy[i].clear(); pg[i].clear();
+      if (in[i] && live) {                              // a row that does not exist adds zeros everywhere
+        const int c = rn_col<L, V>(i, lit);
+        px[i].load(xrow + c);
+        if (a.f) pf[i].load(frow + c);
+        if (a.dr) pdr[i].load(drrow + c);
+        if (a.dy) pdy[i].load(dyrow + c);
+        if (full) pg[i].load(static_cast<const TF*>(a.gate) + rr * a.ldg + c);
+      }
+    }
+    const float grow = a.gate_kind == CXG_GATE_ROW && live ? (float)static_cast<const TF*>(a.gate)[rr * a.ldg] : 1.f;
+    float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
+    if (live) st = reinterpret_cast<const float4*>(a.stats)[rr];
+
+    float fh[ITEMS][V], h[ITEMS][V], gt[ITEMS][V], rh[ITEMS][V], g[ITEMS][V];
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      float x[V], f[V], dy[V], gf[V];
+      px[i].widen(x); pf[i].widen(f); pdy[i].widen(dy); pg[i].widen(gf); pdr[i].widen(g[i]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        fh[i][j] = post ? (f[j] - st.x) * st.y : f[j];
+        h[i][j] = post ? fh[i][j] * w1[i][j] + b1[i][j] : f[j];
+        gt[i][j] = full ? gf[j] : grow;                 // the gate as far as it differs between rows
+        const float hg = (full ? h[i][j] * gf[j] : h[i][j] * gc[i][j]);
+        const float r = a.res_scale * x[j] + a.branch_scale * grow * hg;
+        rh[i][j] = (r - st.z) * st.w;
+        const float t = dy[j] * w2[i][j];
+        s[0] += t;
+        s[1] += t * rh[i][j];
+        sums[0][i][j] += dy[j] * rh[i][j];
+        sums[1][i][j] += dy[j];
+      }
+    }
+    if (pre) {
+      team_sum<L, 2>(s, s_red, slot);
+      const float m0 = pre_layer ? s[0] * inv_c : 0.f, m1 = s[1] * inv_c;
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        float dy[V];
+        pdy[i].widen(dy);
+#pragma unroll
+        for (int j = 0; j < V; ++j) g[i][j] += st.w * (dy[j] * w2[i][j] - m0 - rh[i][j] * m1);
+      }
+    }
+    if (a.dx && live) {
+      TX* const out = static_cast<TX*>(a.dx) + rr * cols;
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i)
+        if (in[i]) {
+          float o[V];
+#pragma unroll
+          for (int j = 0; j < V; ++j) o[j] = a.res_scale * g[i][j];
+          Piece<TX, V> p;
+          p.narrow(o);
+          p.store(out + rn_col<L, V>(i, lit));
+        }
+    }
+    if (a.dgate) {
+      if (full) {
+        if (live) {
+          TF* const out = static_cast<TF*>(a.dgate) + rr * cols;
+#pragma unroll
+          for (int i = 0; i < ITEMS; ++i)
+            if (in[i]) {
+              float o[V];
+#pragma unroll
+              for (int j = 0; j < V; ++j) o[j] = a.branch_scale * g[i][j] * h[i][j];
+              Piece<TF, V> p;
+              p.narrow(o);
+              p.store(out + rn_col<L, V>(i, lit));
+            }
+        }
+      } else if (a.gate_kind == CXG_GATE_ROW) {
+        float d[1] = {0.f};
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+          for (int j = 0; j < V; ++j) d[0] += in[i] ? g[i][j] * h[i][j] : 0.f;
+        team_sum<L, 1>(d, s_red, slot);
+        if (live && lit == 0) static_cast<TF*>(a.dgate)[rr] = (TF)(a.branch_scale * d[0]);
+      }
+    }
+    if (a.f) {
+      float q[2] = {0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float cg = live ? gt[i][j] * g[i][j] : 0.f;
+          sums[2][i][j] += cg * fh[i][j];
+          sums[3][i][j] += cg;
+          g[i][j] = a.branch_scale * cg * (full ? 1.f : gc[i][j]) * w1[i][j];
+          q[0] += g[i][j];
+          q[1] += g[i][j] * fh[i][j];
+        }
+      if (a.df) {
+        float m0 = 0.f, m1 = 0.f;
+        if (post) {
+          team_sum<L, 2>(q, s_red, slot);
+          m0 = post_layer ? q[0] * inv_c : 0.f;
+          m1 = q[1] * inv_c;
+        }
+        if (live) {
+          TF* const out = static_cast<TF*>(a.df) + rr * cols;
+#pragma unroll
+          for (int i = 0; i < ITEMS; ++i)
+            if (in[i]) {
+              float o[V];
+#pragma unroll
+              for (int j = 0; j < V; ++j) o[j] = post ? st.y * (g[i][j] - m0 - fh[i][j] * m1) : g[i][j];
+              Piece<TF, V> p;
+              p.narrow(o);
+              p.store(out + rn_col<L, V>(i, lit));
+            }
+        }
+      }
+    }
+  }
+
+  // the block's partial row: teams of a wave in registers, waves in LDS
+  if (a.partial == nullptr) return;
+  float* const out = a.partial + (size_t)blockIdx.x * kRnSums * cols;
+  if constexpr (L >= kRnThreads) {
+#pragma unroll
+    for (int q = 0; q < kRnSums; ++q)
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const int c = rn_col<L, V>(i, lit) + j;
+          if (c < cols) out[(size_t)q * cols + c] = sums[q][i][j];
+        }
+  } else {
+    constexpr int kWaves = kRnThreads / CXG_WAVE, kWidth = L * V * ITEMS;
+    __shared__ float s_col[kWaves][kWidth];
+#pragma unroll
+    for (int q = 0; q < kRnSums; ++q) {
+      if (q) __syncthreads();
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float t = groups_sum<L>(sums[q][i][j]);
+          if ((threadIdx.x & (CXG_WAVE - 1)) < L) s_col[threadIdx.x >> 6][rn_col<L, V>(i, lit) + j] = t;
+        }
+      __syncthreads();
+      for (int c = threadIdx.x; c < cols; c += kRnThreads)
+        out[(size_t)q * cols + c] = (s_col[0][c] + s_col[1][c]) + (s_col[2][c] + s_col[3][c]);
+    }
+  }
+}
+
+// Partial rows of all blocks -> the gradients of the vectors.  A block takes kFinCols columns and
+// cuts the partial rows into kFinSlices runs.
+constexpr int kFinCols = 16, kFinSlices = 16;
+
+struct RnFinal {
+  const float* partial; int blocks, cols;
+  const float* post_w; const float* post_b; const float* gate;   // gate: channel gate or null
+  float branch_scale;
+  bool post;
+  float* dgate; float* dpost_w; float* dpost_b; float* dpre_w; float* dpre_b;
+};
+
+__global__ __launch_bounds__(kFinCols * kFinSlices) void residual_norm_sums_kernel(RnFinal a) {
+  __shared__ float s[kRnSums][kFinSlices][kFinCols];
+  const int cl = threadIdx.x % kFinCols, slice = threadIdx.x / kFinCols;
+  const int c = blockIdx.x * kFinCols + cl;
+  float acc[kRnSums] = {0.f, 0.f, 0.f, 0.f};
+  if (c < a.cols) {
+    const int per = (a.blocks + kFinSlices - 1) / kFinSlices;
+    const int b1 = (slice + 1) * per < a.blocks ? (slice + 1) * per : a.blocks;
+#pragma unroll 4
+    for (int b = slice * per; b < b1; ++b) {
+      const float* const p = a.partial + (size_t)b * kRnSums * a.cols + c;
+#pragma unroll
+      for (int q = 0; q < kRnSums; ++q) acc[q] += p[(size_t)q * a.cols];
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < kRnSums; ++q) s[q][slice][cl] = acc[q];
+  __syncthreads();
+  if (slice != 0 || c >= a.cols) return;
+#pragma unroll
+  for (int q = 0; q < kRnSums; ++q)
+    for (int k = 1; k < kFinSlices; ++k) acc[q] += s[q][k][cl];
+  const float w = a.post && a.post_w ? a.post_w[c] : 1.f, b = a.post && a.post_b ? a.post_b[c] : 0.f;
+  const float scale = a.branch_scale * (a.gate ? a.gate[c] : 1.f);
+  if (a.dpre_w) a.dpre_w[c] = acc[0];
+  if (a.dpre_b) a.dpre_b[c] = acc[1];
+  if (a.dpost_w) a.dpost_w[c] = scale * acc[2];
+  if (a.dpost_b) a.dpost_b[c] = scale * acc[3];
+  if (a.dgate) a.dgate[c] = a.branch_scale * (w * acc[2] + b * acc[3]);
+}
+
+int64_t bwd_blocks(int64_t rows, int teams) {
+  const int64_t blocks = ceil_div(rows, (int64_t)teams);
+  return blocks > kRnMaxBlocks ? kRnMaxBlocks : blocks;
+}
+
+// launches the row kernel; returns the number of partial rows, or a negative status
+template <typename TX, typename TF, int V, int L, int ITEMS> int launch_bwd(const RnArgs& a, hipStream_t st) {
+  const int64_t blocks = bwd_blocks(a.rows, kRnThreads / L);
+  hipLaunchKernelGGL((residual_norm_bwd_kernel<TX, TF, V, L, ITEMS>), dim3((unsigned)blocks), dim3(kRnThreads), 0, st, a);
+  CXG_LAUNCH_CHECK("residual_norm_bwd_kernel");
+  return (int)blocks;
+}
+
+template <typename TX, typename TF> int dispatch_bwd(const RnArgs& a, bool vec, hipStream_t st) {
+  constexpr int W = 16 / (sizeof(TX) > sizeof(TF) ? sizeof(TX) : sizeof(TF));
+  const int n = vec ? a.cols / W : a.cols;
+  if (vec) {
+    if (n <= 8) return launch_bwd<TX, TF, W, 8, 1>(a, st);
+    if (n <= 16) return launch_bwd<TX, TF, W, 8, 2>(a, st);
+    if (n <= 32) return launch_bwd<TX, TF, W, 16, 2>(a, st);
+    if (n <= 64) return launch_bwd<TX, TF, W, 32, 2>(a, st);
+    if (n <= 128) return launch_bwd<TX, TF, W, 64, 2>(a, st);
+    if (n <= 512) return launch_bwd<TX, TF, W, 256, 2>(a, st);
+    if (n <= 1024) return launch_bwd<TX, TF, W, 256, 4>(a, st);
+    if constexpr (W == 4) return launch_bwd<TX, TF, W, 256, 8>(a, st);
+  } else {
+    if (n <= 16) return launch_bwd<TX, TF, 1, 8, 2>(a, st);
+    if (n <= 64) return launch_bwd<TX, TF, 1, 16, 4>(a, st);
+    if (n <= 256) return launch_bwd<TX, TF, 1, 64, 4>(a, st);
+    if (n <= 1024) return launch_bwd<TX, TF, 1, 256, 4>(a, st);
+    return launch_bwd<TX, TF, 1, 256, 32>(a, st);
+  }
+  return set_error(CXG_ERR_UNSUPPORTED, "rows of more than %d columns", kRnMaxCols);
+}
+
+int dispatch_bwd_types(const RnArgs& a, int stream_type, int branch_type, bool vec, hipStream_t st) {
+  CXG_RN_TYPES(dispatch_bwd)
+  return set_error(CXG_ERR_UNSUPPORTED, "unsupported types");
+}
+
+}  // namespace
+}  // namespace cxg
+
+extern "C" {
+
+size_t cxg_residual_norm_workspace_bytes(int64_t rows, int cols) {
+  if (rows < 0 || cols < 1) return 0;
+  return (size_t)cxg::bwd_blocks(rows, 1) * cxg::kRnSums * (size_t)cols * sizeof(float) + 256;
+}
+
+int cxg_residual_norm_bwd(const void* x, int64_t ldx, const void* f, int64_t ldf, const void* gate, int64_t ldg,
+                          int gate_kind, int post_kind, const float* post_w, const float* post_b, int pre_kind,
+                          const float* pre_w, float res_scale, float branch_scale, int64_t rows, int cols,
+                          int stream_type, int branch_type, const float* stats, const void* dr, int64_t lddr,
+                          const void* dy, int64_t lddy, void* dx, void* df, void* dgate, float* dpost_w,
+                          float* dpost_b, float* dpre_w, float* dpre_b, void* workspace, size_t workspace_bytes,
+                          void* stream) {
+  using namespace cxg;
+  RnArgs a{};
+  a.x = x; a.ldx = ldx; a.f = f; a.ldf = ldf; a.gate = gate; a.ldg = ldg;
+  a.gate_kind = gate_kind; a.post_kind = post_kind; a.pre_kind = pre_kind;
+  a.post_w = post_w; a.post_b = post_b; a.pre_w = pre_w;
+  a.res_scale = res_scale; a.branch_scale = branch_scale;
+  a.rows = rows; a.cols = cols; a.stats = const_cast<float*>(stats);
+  a.dr = dr; a.lddr = lddr; a.dy = dy; a.lddy = lddy; a.dx = dx; a.df = df;
+  const int bad = rn_check(a, stream_type, branch_type);
+  if (bad) return bad;
+  CXG_REQUIRE(rows == 0 || (stats && ((uintptr_t)stats & 15) == 0), CXG_ERR_ARG, "stats missing or not 16-byte aligned");
+  CXG_REQUIRE(rows == 0 || f || !df, CXG_ERR_ARG, "a branch gradient needs branch rows");
+  CXG_REQUIRE(!dgate || gate_kind != CXG_GATE_NONE, CXG_ERR_ARG, "a gate gradient needs a gate");
+  const bool channel = gate_kind == CXG_GATE_CHANNEL;
+  const bool sums = dpost_w || dpost_b || dpre_w || dpre_b || (channel && dgate);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  RnFinal fin{};
+  fin.cols = cols;
+  fin.post_w = post_w; fin.post_b = post_b; fin.gate = channel ? static_cast<const float*>(gate) : nullptr;
+  fin.branch_scale = branch_scale;
+  fin.post = post_kind != CXG_NORM_NONE;
+  fin.dgate = channel ? static_cast<float*>(dgate) : nullptr;
+  fin.dpost_w = dpost_w; fin.dpost_b = dpost_b; fin.dpre_w = dpre_w; fin.dpre_b = dpre_b;
+  if (sums) {
+    const size_t need = cxg_residual_norm_workspace_bytes(rows, cols);
+    CXG_REQUIRE(workspace && workspace_bytes >= need, CXG_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need,
+                workspace_bytes);
+    CXG_REQUIRE(((uintptr_t)workspace & 15) == 0, CXG_ERR_WORKSPACE, "workspace must be 16-byte aligned");
+    a.partial = static_cast<float*>(workspace);
+    fin.partial = a.partial;
+  }
+  if (!channel) a.dgate = dgate;
+  if (rows > 0) {
+    const size_t sx = value_bytes(stream_type), sf = value_bytes(branch_type);
+    const int v = stream_type == CXG_F32 || branch_type == CXG_F32 ? 4 : 8;
+    const bool full = gate_kind == CXG_GATE_FULL;
+    const bool vec = cols % v == 0 && rn_aligned(x, ldx, sx, v) && rn_aligned(f, ldf, sf, v) && rn_aligned(dr, lddr, sx, v) &&
+                     rn_aligned(dy, lddy, sf, v) && rn_aligned(dx, 0, sx, v) && rn_aligned(df, 0, sf, v) &&
+                     (!full || (rn_aligned(gate, ldg, sf, v) && rn_aligned(dgate, 0, sf, v)));
+    const int blocks = dispatch_bwd_types(a, stream_type, branch_type, vec, st);
+    if (blocks < 0) return blocks;
+    fin.blocks = blocks;
+  }
+  if (sums) {
+    hipLaunchKernelGGL(residual_norm_sums_kernel, dim3((unsigned)ceil_div(cols, kFinCols)), dim3(kFinCols * kFinSlices), 0,
+                       st, fin);
+    CXG_LAUNCH_CHECK("residual_norm_sums_kernel");
+  }
+  return CXG_OK;
+}
+
+}  // extern "C"

@@ -99,6 +99,11 @@ SIGNATURES = {
     "cxg_batchnorm_apply_f32": (_I32, [_P, _I64, _I32, _I64, _P, _P, _P, _P, _P, _I64, _I32, _P]),
     "cxg_batchnorm_bwd_f32": (_I32, [_P, _P, _I64, _I32, _I64, _I64, _P, _P, _P, _P, _I32, _P, _I64, _P, _P, _P,
                                      _SZ, _P]),
+    "cxg_residual_norm_fwd": (_I32, [_P, _I64, _P, _I64, _P, _I64, _I32, _I32, _P, _P, _I32, _P, _P, _F32, _F32, _F32,
+                                     _I64, _I32, _I32, _I32, _P, _P, _P, _P]),
+    "cxg_residual_norm_workspace_bytes": (_SZ, [_I64, _I32]),
+    "cxg_residual_norm_bwd": (_I32, [_P, _I64, _P, _I64, _P, _I64, _I32, _I32, _P, _P, _I32, _P, _F32, _F32, _I64, _I32,
+                                     _I32, _I32, _P, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
 }
 
 _lib = None

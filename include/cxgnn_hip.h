@@ -732,6 +732,59 @@ int cxg_coo_to_csr_i64(const int64_t* src, const int64_t* dst, int64_t n_edges, 
 int64_t cxg_topo_sort_host_i64(const int64_t* ptr, const int64_t* idx, const int64_t* degree,
                                int64_t n_nodes, int64_t* order);
 
+/* ------------------------------------------------------------------------- */
+/* Residual norm (no counterpart in the reference, whose models normalise over */
+/* the batch only): the connection between the blocks of a deep model          */
+/* ------------------------------------------------------------------------- */
+
+/* value types of rows that may be narrower than fp32 */
+#define CXG_F32 0
+#define CXG_BF16 1
+#define CXG_F16 2
+
+#define CXG_NORM_NONE 0
+#define CXG_NORM_RMS 1    /* v / sqrt(mean(v^2) + eps) * w + b */
+#define CXG_NORM_LAYER 2  /* (v - mean(v)) / sqrt(var(v) + eps) * w + b, biased variance */
+
+#define CXG_GATE_NONE 0
+#define CXG_GATE_CHANNEL 1 /* fp32 [cols]                             */
+#define CXG_GATE_ROW 2     /* branch type, one value per row, stride ldg */
+#define CXG_GATE_FULL 3    /* branch type [rows, cols], row stride ldg   */
+
+/*
+ * r = res_scale * x + branch_scale * gate * post(f),  y = pre(r), row by row over `cols` columns
+ * (at most 8192, otherwise CXG_ERR_UNSUPPORTED).  x and r are of stream_type, f, y and a gate of
+ * rows or elements of branch_type; the two types are equal or the stream is fp32.  The norms'
+ * vectors are fp32 [cols]; a NULL weight is 1, a NULL bias 0.  Statistics and arithmetic are fp32
+ * and y is formed from r before r is rounded.  Row strides in values, 0 for one shared row; r and y
+ * are contiguous.  f NULL: y = pre(res_scale * x), no gate, no post norm, r may be NULL.  pre_kind
+ * CXG_NORM_NONE: y is not written.  stats (NULL where no backward pass follows; 16-byte aligned)
+ * receives [rows][4] = mean and 1/std of the branch row, mean and 1/std of the stream row.
+ */
+int cxg_residual_norm_fwd(const void* x, int64_t ldx, const void* f, int64_t ldf, const void* gate,
+                          int64_t ldg, int gate_kind, int post_kind, const float* post_w,
+                          const float* post_b, int pre_kind, const float* pre_w, const float* pre_b,
+                          float res_scale, float branch_scale, float eps, int64_t rows, int cols,
+                          int stream_type, int branch_type, void* r, void* y, float* stats,
+                          void* stream);
+
+/*
+ * Its backward pass: gradients of x, f, the gate and the norms' vectors from dr and dy (either may
+ * be NULL = zeros), the inputs of the forward call and its stats.  Every output may be NULL; dx, df
+ * and an element-wise dgate are contiguous, a channel gate's dgate is fp32 [cols], the vectors'
+ * gradients fp32 [cols].  The workspace (16-byte aligned) is needed for sums over rows only.  Sums
+ * are added in a fixed order: results repeat bit for bit.  No rows: vector gradients are 0.
+ */
+size_t cxg_residual_norm_workspace_bytes(int64_t rows, int cols);
+int cxg_residual_norm_bwd(const void* x, int64_t ldx, const void* f, int64_t ldf, const void* gate,
+                          int64_t ldg, int gate_kind, int post_kind, const float* post_w,
+                          const float* post_b, int pre_kind, const float* pre_w, float res_scale,
+                          float branch_scale, int64_t rows, int cols, int stream_type,
+                          int branch_type, const float* stats, const void* dr, int64_t lddr,
+                          const void* dy, int64_t lddy, void* dx, void* df, void* dgate,
+                          float* dpost_w, float* dpost_b, float* dpre_w, float* dpre_b,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
