@@ -218,9 +218,12 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_bwd_kernel(RnArgs a)
   }
 }
 
-// Partial rows of all blocks -> the gradients of the vectors.  A block takes kFinCols columns and
-// cuts the partial rows into kFinSlices runs.
-constexpr int kFinCols = 16, kFinSlices = 16;
+// Partial rows of all blocks -> the gradients of the vectors.  A block of 1024 threads takes
+// kFinCols columns: a thread adds one of the four sums of a column over one of kFinSlices runs of
+// partial rows, the runs are added across lanes.  (256 threads per 16 columns, four sums per thread
+// and 16 runs: 14 us for 1024 partial rows of 256 columns, latency of 64 dependent steps.)
+constexpr int kFinCols = 8, kFinSlices = 32;
+constexpr int kFinThreads = kFinCols * kFinSlices * kRnSums;
 
 struct RnFinal {
   const float* partial; int blocks, cols;
@@ -230,35 +233,35 @@ struct RnFinal {
   float* dgate; float* dpost_w; float* dpost_b; float* dpre_w; float* dpre_b;
 };
 
-__global__ __launch_bounds__(kFinCols * kFinSlices) void residual_norm_sums_kernel(RnFinal a) {
-  __shared__ float s[kRnSums][kFinSlices][kFinCols];
-  const int cl = threadIdx.x % kFinCols, slice = threadIdx.x / kFinCols;
-  const int c = blockIdx.x * kFinCols + cl;
-  float acc[kRnSums] = {0.f, 0.f, 0.f, 0.f};
-  if (c < a.cols) {
+__global__ __launch_bounds__(kFinThreads) void residual_norm_sums_kernel(RnFinal a) {
+  constexpr int kPairs = kRnSums * kFinCols;
+  __shared__ float s[kFinSlices][kPairs + 1], s_out[kPairs];
+  const int cl = threadIdx.x % kFinCols, q = (threadIdx.x / kFinCols) % kRnSums, slice = threadIdx.x / kPairs;
+  const int c0 = blockIdx.x * kFinCols;
+  float acc = 0.f;
+  if (c0 + cl < a.cols) {
     const int per = (a.blocks + kFinSlices - 1) / kFinSlices;
     const int b1 = (slice + 1) * per < a.blocks ? (slice + 1) * per : a.blocks;
-#pragma unroll 4
-    for (int b = slice * per; b < b1; ++b) {
-      const float* const p = a.partial + (size_t)b * kRnSums * a.cols + c;
-#pragma unroll
-      for (int q = 0; q < kRnSums; ++q) acc[q] += p[(size_t)q * a.cols];
-    }
+    const float* const p = a.partial + (size_t)q * a.cols + c0 + cl;
+#pragma unroll 8
+    for (int b = slice * per; b < b1; ++b) acc += p[(size_t)b * kRnSums * a.cols];
   }
-#pragma unroll
-  for (int q = 0; q < kRnSums; ++q) s[q][slice][cl] = acc[q];
+  s[slice][q * kFinCols + cl] = acc;
   __syncthreads();
-  if (slice != 0 || c >= a.cols) return;
-#pragma unroll
-  for (int q = 0; q < kRnSums; ++q)
-    for (int k = 1; k < kFinSlices; ++k) acc[q] += s[q][k][cl];
+  static_assert(kFinSlices == 32 && kFinThreads / kFinSlices == kPairs, "half a wave per sum");
+  const float total = lanes_sum<kFinSlices>(s[threadIdx.x % kFinSlices][threadIdx.x / kFinSlices]);
+  if (threadIdx.x % kFinSlices == 0) s_out[threadIdx.x / kFinSlices] = total;
+  __syncthreads();
+  const int c = c0 + threadIdx.x;
+  if (threadIdx.x >= kFinCols || c >= a.cols) return;
+  const float s0 = s_out[cl], s1 = s_out[kFinCols + cl], s2 = s_out[2 * kFinCols + cl], s3 = s_out[3 * kFinCols + cl];
   const float w = a.post && a.post_w ? a.post_w[c] : 1.f, b = a.post && a.post_b ? a.post_b[c] : 0.f;
   const float scale = a.branch_scale * (a.gate ? a.gate[c] : 1.f);
-  if (a.dpre_w) a.dpre_w[c] = acc[0];
-  if (a.dpre_b) a.dpre_b[c] = acc[1];
-  if (a.dpost_w) a.dpost_w[c] = scale * acc[2];
-  if (a.dpost_b) a.dpost_b[c] = scale * acc[3];
-  if (a.dgate) a.dgate[c] = a.branch_scale * (w * acc[2] + b * acc[3]);
+  if (a.dpre_w) a.dpre_w[c] = s0;
+  if (a.dpre_b) a.dpre_b[c] = s1;
+  if (a.dpost_w) a.dpost_w[c] = scale * s2;
+  if (a.dpost_b) a.dpost_b[c] = scale * s3;
+  if (a.dgate) a.dgate[c] = a.branch_scale * (w * s2 + b * s3);
 }
 
 int64_t bwd_blocks(int64_t rows, int teams) {
@@ -362,7 +365,7 @@ int cxg_residual_norm_bwd(const void* x, int64_t ldx, const void* f, int64_t ldf
     fin.blocks = blocks;
   }
   if (sums) {
-    hipLaunchKernelGGL(residual_norm_sums_kernel, dim3((unsigned)ceil_div(cols, kFinCols)), dim3(kFinCols * kFinSlices), 0,
+    hipLaunchKernelGGL(residual_norm_sums_kernel, dim3((unsigned)ceil_div(cols, kFinCols)), dim3(kFinThreads), 0,
                        st, fin);
     CXG_LAUNCH_CHECK("residual_norm_sums_kernel");
   }

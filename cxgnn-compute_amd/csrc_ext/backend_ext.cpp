@@ -942,6 +942,221 @@ void spmm_multihead_bwd(const Tensor& ptr, const Tensor& idx, const Tensor& val,
   spmm(g->ptr_t, g->idx_t, grad_output.contiguous(), grad_x.size(0), false, val, g->perm, grad_x, true, c10::nullopt);
 }
 
+// ---------------------------------------------------------------------------------------------
+// residual norm: r = res_scale * x + branch_scale * gate * post(f), y = pre(r)
+// (cxg_residual_norm_fwd / _bwd; no counterpart in the reference)
+// ---------------------------------------------------------------------------------------------
+int value_type(const Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return CXG_F32;
+    case at::kBFloat16: return CXG_BF16;
+    case at::kHalf: return CXG_F16;
+    default: bad(fmt("%s must be float32, bfloat16 or float16, got %s", name, dtype_name(t.scalar_type())));
+  }
+}
+
+// A device matrix whose rows are contiguous (their stride is free), copied if they are not.
+Tensor rows_of(const Tensor& t, const char* name) {
+  if (!t.defined()) bad(fmt("%s must be a tensor", name));
+  if (!t.is_cuda()) bad(fmt("%s must be a CUDA tensor", name));
+  value_type(t, name);
+  if (t.dim() != 2) bad(fmt("%s must have 2 dims, got %d", name, (int)t.dim()));
+  return t.stride(1) == 1 || t.size(1) == 1 ? t : t.contiguous();
+}
+
+void same_device(const Tensor& t, const Tensor& x, const char* name) {
+  if (t.device() != x.device()) bad(fmt("%s is on %s, expected %s", name, t.device().str().c_str(), x.device().str().c_str()));
+}
+
+int norm_kind(const c10::optional<std::string>& kind, const char* name) {
+  if (!kind.has_value()) return CXG_NORM_NONE;
+  if (*kind == "rms") return CXG_NORM_RMS;
+  if (*kind == "layer") return CXG_NORM_LAYER;
+  bad(fmt("%s must be 'layer', 'rms' or None, got '%s'", name, kind->c_str()));
+}
+
+enum RnTensor { kRnX, kRnF, kRnGate, kRnPostW, kRnPostB, kRnPreW, kRnPreB, kRnTensors };
+
+// The checked arguments of one call; tensors that are missing are undefined.
+struct ResidualNorm {
+  Tensor t[kRnTensors];
+  int gate_kind = CXG_GATE_NONE, post = 0, pre = 0, stream_type = 0, branch_type = 0;
+  double res_scale = 1, branch_scale = 1, eps = 0;
+  int64_t rows = 0, cols = 0;
+  at::ScalarType branch_dtype = at::kFloat;
+
+  const float* vec(int i) const { return t[i].defined() ? (const float*)t[i].data_ptr() : nullptr; }
+  const void* ptr(int i) const { return t[i].defined() ? t[i].data_ptr() : nullptr; }
+  int64_t ld(int i) const { return t[i].defined() && t[i].dim() == 2 ? t[i].stride(0) : 0; }
+  Tensor matrix(at::ScalarType dtype) const { return torch::empty({rows, cols}, t[kRnX].options().dtype(dtype).requires_grad(false)); }
+};
+
+void rn_vector(Tensor& v, const char* name, const ResidualNorm& c) {
+  if (!v.defined()) return;
+  if (v.scalar_type() != at::kFloat || v.dim() != 1 || v.size(0) != c.cols)
+    bad(fmt("%s must be float32 [%lld], got %s of %d dims", name, (long long)c.cols, dtype_name(v.scalar_type()), (int)v.dim()));
+  same_device(v, c.t[kRnX], name);
+  v = v.contiguous();
+}
+
+void rn_prepare(ResidualNorm& c) {
+  Tensor &x = c.t[kRnX], &f = c.t[kRnF], &gate = c.t[kRnGate];
+  x = rows_of(x, "x");
+  c.rows = x.size(0);
+  c.cols = x.size(1);
+  if (c.cols < 1 || c.cols > 8192) bad(fmt("residual_norm takes 1 to 8192 columns, got %lld", (long long)c.cols));
+  if (f.defined()) {
+    f = rows_of(f, "f");
+    same_device(f, x, "f");
+    if (f.sizes() != x.sizes()) bad("f and x differ in shape");
+    if (x.scalar_type() != at::kFloat && f.scalar_type() != x.scalar_type())
+      bad(fmt("f must have x's dtype %s unless x is float32, got %s", dtype_name(x.scalar_type()), dtype_name(f.scalar_type())));
+  } else if (gate.defined() || c.post != CXG_NORM_NONE || c.res_scale != 1.0 || c.pre == CXG_NORM_NONE) {
+    bad("without a branch there is the norm of x alone: no gate, post norm or scale, and a pre norm");
+  }
+  c.branch_dtype = f.defined() ? f.scalar_type() : x.scalar_type();
+  c.stream_type = value_type(x, "x");
+  c.branch_type = f.defined() ? value_type(f, "f") : c.stream_type;
+  if (c.post == CXG_NORM_NONE && (c.t[kRnPostW].defined() || c.t[kRnPostB].defined())) bad("post_weight / post_bias without a post norm");
+  if (c.pre == CXG_NORM_NONE && (c.t[kRnPreW].defined() || c.t[kRnPreB].defined())) bad("pre_weight / pre_bias without a pre norm");
+  rn_vector(c.t[kRnPostW], "post_weight", c);
+  rn_vector(c.t[kRnPostB], "post_bias", c);
+  rn_vector(c.t[kRnPreW], "pre_weight", c);
+  rn_vector(c.t[kRnPreB], "pre_bias", c);
+  if (!gate.defined()) {
+    c.gate_kind = CXG_GATE_NONE;
+  } else if (gate.dim() == 1) {
+    rn_vector(gate, "a gate of columns", c);
+    c.gate_kind = CXG_GATE_CHANNEL;
+  } else {
+    gate = rows_of(gate, "gate");
+    same_device(gate, x, "gate");
+    if (gate.scalar_type() != c.branch_dtype)
+      bad(fmt("a gate of rows or elements has f's dtype %s, got %s", dtype_name(c.branch_dtype), dtype_name(gate.scalar_type())));
+    if (gate.size(0) == c.rows && gate.size(1) == 1) c.gate_kind = CXG_GATE_ROW;
+    else if (gate.size(0) == c.rows && gate.size(1) == c.cols) c.gate_kind = CXG_GATE_FULL;
+    else bad(fmt("gate must be [%lld], [%lld, 1] or [%lld, %lld]", (long long)c.cols, (long long)c.rows, (long long)c.rows, (long long)c.cols));
+  }
+}
+
+void rn_forward(const ResidualNorm& c, Tensor& r, Tensor& y, Tensor* stats) {
+  if (c.t[kRnF].defined()) r = c.matrix(c.t[kRnX].scalar_type());
+  if (c.pre != CXG_NORM_NONE) y = c.matrix(c.branch_dtype);
+  if (stats) *stats = torch::empty({c.rows, 4}, c.t[kRnX].options().dtype(at::kFloat).requires_grad(false));
+  c10::DeviceGuard guard(c.t[kRnX].device());
+  check(cxg_residual_norm_fwd(c.ptr(kRnX), c.ld(kRnX), c.ptr(kRnF), c.ld(kRnF), c.ptr(kRnGate), c.ld(kRnGate), c.gate_kind, c.post,
+                              c.vec(kRnPostW), c.vec(kRnPostB), c.pre, c.vec(kRnPreW), c.vec(kRnPreB), (float)c.res_scale,
+                              (float)c.branch_scale, (float)c.eps, c.rows, (int)c.cols, c.stream_type, c.branch_type,
+                              r.defined() ? r.data_ptr() : nullptr, y.defined() ? y.data_ptr() : nullptr,
+                              stats ? (float*)stats->data_ptr() : nullptr, stream_of(c.t[kRnX])));
+}
+
+struct ResidualNormFunction : public torch::autograd::Function<ResidualNormFunction> {
+  static tensor_list forward(AutogradContext* ctx, Tensor x, OptTensor f, OptTensor gate, OptTensor post_w, OptTensor post_b,
+                             OptTensor pre_w, OptTensor pre_b, int64_t post, int64_t pre, double res_scale, double branch_scale,
+                             double eps) {
+    const OptTensor given[kRnTensors] = {x, f, gate, post_w, post_b, pre_w, pre_b};
+    ResidualNorm c;
+    std::vector<int64_t> need;
+    for (int i = 0; i < kRnTensors; ++i) {
+      if (given[i].has_value()) c.t[i] = *given[i];
+      need.push_back(c.t[i].defined() && c.t[i].requires_grad());
+    }
+    c.post = (int)post; c.pre = (int)pre;
+    c.res_scale = res_scale; c.branch_scale = branch_scale; c.eps = eps;
+    tensor_list saved(c.t, c.t + kRnTensors);      // the caller's own tensors: a change in place is noticed
+    rn_prepare(c);
+    Tensor r, y, stats;
+    rn_forward(c, r, y, &stats);
+    saved.push_back(stats);
+    ctx->save_for_backward(saved);
+    ctx->saved_data["how"] = std::vector<int64_t>{post, pre};
+    ctx->saved_data["scales"] = std::vector<double>{res_scale, branch_scale, eps};
+    ctx->saved_data["need"] = need;
+    ctx->set_materialize_grads(false);
+    tensor_list out;
+    if (r.defined()) out.push_back(r);
+    if (y.defined()) out.push_back(y);
+    return out;
+  }
+
+  static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+    if (at::GradMode::is_enabled()) throw std::runtime_error("residual_norm has no second derivatives (create_graph=True)");
+    const auto saved = ctx->get_saved_variables();
+    const std::vector<int64_t> how = ctx->saved_data["how"].toIntVector(), need = ctx->saved_data["need"].toIntVector();
+    const std::vector<double> scales = ctx->saved_data["scales"].toDoubleVector();
+    ResidualNorm c;
+    for (int i = 0; i < kRnTensors; ++i) c.t[i] = saved[i];
+    c.post = (int)how[0]; c.pre = (int)how[1];
+    c.res_scale = scales[0]; c.branch_scale = scales[1]; c.eps = scales[2];
+    rn_prepare(c);
+    const Tensor& stats = saved[kRnTensors];
+    const bool has_r = c.t[kRnF].defined();
+    Tensor dr = has_r ? grads[0] : Tensor(), dy = c.pre != CXG_NORM_NONE ? grads[has_r ? 1 : 0] : Tensor();
+    tensor_list out(12);
+    if (!dr.defined() && !dy.defined()) return out;
+    if (dr.defined()) dr = rows_of(dr, "the gradient of r");
+    if (dy.defined()) dy = rows_of(dy, "the gradient of y");
+    const auto fp32 = stats.options();
+    if (need[kRnX]) out[kRnX] = c.matrix(c.t[kRnX].scalar_type());
+    if (need[kRnF]) out[kRnF] = c.matrix(c.branch_dtype);
+    if (need[kRnGate])
+      out[kRnGate] = c.gate_kind == CXG_GATE_CHANNEL ? torch::empty({c.cols}, fp32)
+                                                     : torch::empty(c.t[kRnGate].sizes(), fp32.dtype(c.branch_dtype));
+    bool sums = need[kRnGate] && c.gate_kind == CXG_GATE_CHANNEL;
+    for (int i = kRnPostW; i < kRnTensors; ++i)
+      if (need[i]) {
+        out[i] = torch::empty({c.cols}, fp32);
+        sums = true;
+      }
+    Tensor ws;
+    if (sums) ws = workspace(cxg_residual_norm_workspace_bytes(c.rows, (int)c.cols), stats);
+    auto at = [&](int i) { return out[i].defined() ? out[i].data_ptr() : nullptr; };
+    c10::DeviceGuard guard(stats.device());
+    check(cxg_residual_norm_bwd(c.ptr(kRnX), c.ld(kRnX), c.ptr(kRnF), c.ld(kRnF), c.ptr(kRnGate), c.ld(kRnGate), c.gate_kind, c.post,
+                                c.vec(kRnPostW), c.vec(kRnPostB), c.pre, c.vec(kRnPreW), (float)c.res_scale, (float)c.branch_scale,
+                                c.rows, (int)c.cols, c.stream_type, c.branch_type, (const float*)stats.data_ptr(),
+                                dr.defined() ? dr.data_ptr() : nullptr, dr.defined() ? dr.stride(0) : 0,
+                                dy.defined() ? dy.data_ptr() : nullptr, dy.defined() ? dy.stride(0) : 0, at(kRnX), at(kRnF), at(kRnGate),
+                                (float*)at(kRnPostW), (float*)at(kRnPostB), (float*)at(kRnPreW), (float*)at(kRnPreB),
+                                sums ? ws.data_ptr() : nullptr, sums ? (size_t)ws.numel() : 0, stream_of(stats)));
+    return out;
+  }
+};
+
+// (r, y): r None without a branch, y None without a pre norm
+std::tuple<OptTensor, OptTensor> residual_norm(const Tensor& x, const OptTensor& f, const OptTensor& gate,
+                                               const c10::optional<std::string>& post, const OptTensor& post_w, const OptTensor& post_b,
+                                               const c10::optional<std::string>& pre, const OptTensor& pre_w, const OptTensor& pre_b,
+                                               double res_scale, double branch_scale, double eps) {
+  ResidualNorm c;
+  const OptTensor given[kRnTensors] = {x, f, gate, post_w, post_b, pre_w, pre_b};
+  c.post = norm_kind(post, "post");
+  c.pre = norm_kind(pre, "pre");
+  bool grad = false;
+  for (int i = 0; i < kRnTensors; ++i)
+    if (given[i].has_value() && given[i]->defined()) {
+      c.t[i] = *given[i];
+      grad = grad || c.t[i].requires_grad();
+    }
+  OptTensor r, y;
+  if (grad && at::GradMode::is_enabled()) {
+    const tensor_list out = ResidualNormFunction::apply(x, f, gate, post_w, post_b, pre_w, pre_b, (int64_t)c.post, (int64_t)c.pre,
+                                                        res_scale, branch_scale, eps);
+    const bool has_r = c.t[kRnF].defined();
+    if (has_r) r = out[0];
+    if (c.pre != CXG_NORM_NONE) y = out[has_r ? 1 : 0];
+    return std::make_tuple(r, y);
+  }
+  c.res_scale = res_scale; c.branch_scale = branch_scale; c.eps = eps;
+  rn_prepare(c);
+  Tensor rt, yt;
+  rn_forward(c, rt, yt, nullptr);
+  if (rt.defined()) r = rt;
+  if (yt.defined()) y = yt;
+  return std::make_tuple(r, y);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -963,6 +1178,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("val") = py::none(), py::arg("val_perm") = py::none(), py::arg("out") = py::none(),
         py::arg("accumulate") = false, py::arg("bias") = py::none());
   m.def("head_sum", &head_sum);
+  m.def("residual_norm", &residual_norm, py::arg("x"), py::arg("f"), py::arg("gate"), py::arg("post"), py::arg("post_weight"),
+        py::arg("post_bias"), py::arg("pre"), py::arg("pre_weight"), py::arg("pre_bias"), py::arg("res_scale"),
+        py::arg("branch_scale"), py::arg("eps"));
   m.def("edge_value_degree_raw", &edge_value_degree);
   m.def("sddmm_csr", &sddmm_csr, py::arg("ptr"), py::arg("idx"), py::arg("src_feat"), py::arg("dst_feat"),
         py::arg("n_rows"), py::arg("out") = py::none());

@@ -21,7 +21,7 @@ from .batch import Batch, PyGBatch
 from .util import global_tuner
 from .graph_kernel import SpMMValOP
 from .batchnorm import BatchNorm1d
-from .residual import ResidualNorm, ResidualNormOP, residual_norm
+from .residual import ResidualNorm, residual_norm
 from .model import (GNN, SAGE, GCN, GIN, GAT, RGCN, get_model, get_conv_from_str, get_model_from_str,
                     graph_type_dict, model_dict)
 from . import synthetic  # noqa: F401

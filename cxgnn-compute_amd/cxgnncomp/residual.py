@@ -9,36 +9,10 @@ The batch norm of the models (``BatchNorm1d``) stays what it is; these norms wor
 itself.  No counterpart upstream.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
-from cxgnncomp_backend import _residual
+from cxgnncomp_backend import residual_norm as _residual_norm
 
-
-class ResidualNormOP(torch.autograd.Function):
-    """``residual_norm`` as one autograd node: the backward pass reads x, f, the gate and two
-    statistics per norm and row; r and y are not kept."""
-
-    @staticmethod
-    def forward(ctx, x, f, gate, post_weight, post_bias, pre_weight, pre_bias, post, pre, res_scale, branch_scale, eps):
-        call = _residual.Call(x, f, gate, post, post_weight, post_bias, pre, pre_weight, pre_bias, res_scale,
-                              branch_scale, eps)
-        r, y, stats = _residual.forward(call, True)
-        ctx.save_for_backward(x, f, gate, post_weight, post_bias, pre_weight, pre_bias, stats)
-        ctx.how = (post, pre, res_scale, branch_scale, eps)
-        ctx.set_materialize_grads(False)
-        return r, y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dr, dy):
-        x, f, gate, post_weight, post_bias, pre_weight, pre_bias, stats = ctx.saved_tensors
-        post, pre, res_scale, branch_scale, eps = ctx.how
-        need = ctx.needs_input_grad[:7]
-        if dr is None and dy is None:
-            return (None, ) * 12
-        call = _residual.Call(x, f, gate, post, post_weight, post_bias, pre, pre_weight, pre_bias, res_scale,
-                              branch_scale, eps)
-        return _residual.backward(call, stats, dr, dy, need) + (None, ) * 5
+_KINDS = (None, "layer", "rms")
 
 
 def residual_norm(x, f, gate=None, *, post=None, post_weight=None, post_bias=None, pre="layer", pre_weight=None,
@@ -54,16 +28,12 @@ def residual_norm(x, f, gate=None, *, post=None, post_weight=None, post_bias=Non
 
     ``f=None`` (the entry of a stack, before any block): ``(x, pre(x))``, x itself.
 
-    Gradients of every tensor argument, once (no second derivatives); the sums over rows behind the
+    One autograd node (csrc_ext/backend_ext.cpp): its backward pass reads x, f, the gate and two
+    statistics per norm and row; r and y are not kept.  Gradients of every tensor argument, once (no
+    second derivatives); the sums over rows behind the
     vectors' gradients are added in a fixed order, so they repeat bit for bit.
     """
-    tensors = (x, f, gate, post_weight, post_bias, pre_weight, pre_bias)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors if isinstance(t, torch.Tensor)):
-        r, y = ResidualNormOP.apply(*tensors, post, pre, res_scale, branch_scale, eps)
-    else:
-        call = _residual.Call(x, f, gate, post, post_weight, post_bias, pre, pre_weight, pre_bias, res_scale,
-                              branch_scale, eps)
-        r, y, _ = _residual.forward(call, False)
+    r, y = _residual_norm(x, f, gate, post, post_weight, post_bias, pre, pre_weight, pre_bias, res_scale, branch_scale, eps)
     return (x if f is None else r), y
 
 
@@ -80,7 +50,7 @@ class ResidualNorm(torch.nn.Module):
         if gate not in (None, "channel"):
             raise ValueError("gate must be None or 'channel', got %r" % (gate, ))
         for kind, name in ((post, "post"), (pre, "pre")):
-            if kind not in _residual.NORM_KINDS:
+            if kind not in _KINDS:
                 raise ValueError("%s must be 'layer', 'rms' or None, got %r" % (name, kind))
         self.channels, self.post, self.pre = channels, post, pre
         self.gate_init, self.res_scale, self.branch_scale, self.eps = gate_init, res_scale, branch_scale, eps

@@ -62,6 +62,9 @@ spmv = _C.spmv
 # binding.cpp:19); autograd in C++, destination groups cached per destination array
 gather = _C.gather
 
+# r = res_scale * x + branch_scale * gate * post(f), y = pre(r): one node, no counterpart upstream
+residual_norm = _C.residual_norm
+
 from ._rel import (aggr_rel, selective_aggr, selective_aggr_bwd, target_aggr,  # noqa: E402,F401
                    target_aggr_backward)
 from ._typed import (aggr_rel_direct, aggr_rgcn_direct_func, aggr_rgcn_mean, pad_rel, pad_rel_idx,  # noqa: E402,F401
