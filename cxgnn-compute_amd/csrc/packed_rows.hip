@@ -1,0 +1,220 @@
+// Rows held in 8 bits: what a layer keeps of its input for the backward pass.
+//
+//   128 consecutive columns of a row share a scale 2^k;  code = x * 2^-k rounded to the nearest (ties to even)
+//   int8: |code| <= 127     e4m3: |code| <= 448 (float8 e4m3fn)     k: the smallest exponent with which the
+//   group's largest magnitude fits after rounding, at least -111
+//
+// A power of two makes both directions exact but for the one rounding: x * 2^-k and code * 2^k are
+// representable, so packing what was unpacked returns the same codes, and code * 2^k is a bf16
+// number (8 significant bits), which is what the matrix kernel that reads these rows needs
+// (packed_wgrad.hip).  int8 keeps 7 bits below the group's largest power of two, e4m3 keeps 3 bits
+// of every value down to 2^-6 * 2^k: the first for even rows, the second for rows of a wide range.
+// A group with an infinity or a NaN has exponent byte 255 and codes 0: it reads back as NaN.
+//
+// Layout: codes [rows][pitch] with the columns rounded up to 16 (zeros behind the last), one
+// exponent byte k + 127 per group, [rows][groups].
+//
+// Bound: memory, one pass.  Eight lanes own a group and hold its 128 values in registers between the
+// maximum (integer maxima of the magnitudes' bits, so that a NaN is largest; three data-parallel
+// moves) and the rounding; a piece of the group is 128 contiguous bytes over the eight lanes.
+#include "packed_rows.hpp"
+
+namespace cxg {
+namespace {
+
+constexpr int kPrThreads = 256;
+constexpr int kPrLanes = 8;                              // lanes per group
+constexpr int kPrTeams = kPrThreads / kPrLanes;          // rows per block step
+
+struct PackArgs {
+  const void* x; int64_t ldx;
+  uint8_t* codes; uint8_t* exps;
+  void* out;
+  int64_t rows;
+  int cols, pitch, groups;
+};
+
+template <int CTRL> __device__ __forceinline__ unsigned moved_max(unsigned m) {
+  const unsigned o = (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, CTRL, 0xf, 0xf, false);
+  return o > m ? o : m;
+}
+
+// Exponent byte of a group from the bits of its largest magnitude.
+template <int FMT> __device__ __forceinline__ int exponent_byte(unsigned top) {
+  const int e = (int)(top >> 23), man = (int)(top & 0x7fffffu);
+  int b;
+  if constexpr (FMT == CXG_PACK_INT8) b = e - 6 + (man >= 0x7f0000 ? 1 : 0);     // 127.5 / 64 and more would round to 128
+  else b = e - 8 + (man > 0x600000 ? 1 : 0);                                     // 448 = 1.75 * 2^8
+  b = b < kPrMinExp ? kPrMinExp : b;
+  return e == 255 ? kPrNotFinite : b;
+}
+
+// Four values times 2^-k as four codes in one register.
+template <int FMT> __device__ __forceinline__ unsigned encode4(const float* v, float inv) {
+  if constexpr (FMT == CXG_PACK_INT8) {
+    // added to 1.5 * 2^23 the product rounds to an integer, which then is the low byte of the sum
+    unsigned t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = __float_as_uint(__builtin_fmaf(v[i], inv, 12582912.f));
+    const unsigned lo = __builtin_amdgcn_perm(t[1], t[0], 0x0c0c0400), hi = __builtin_amdgcn_perm(t[3], t[2], 0x0c0c0400);
+    return __builtin_amdgcn_perm(hi, lo, 0x05040100);
+  } else {
+    int t = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, t, true);
+  }
+}
+
+template <typename T, int FMT> __global__ __launch_bounds__(kPrThreads) void pack_rows_kernel(PackArgs a) {
+  constexpr int V = 16 / sizeof(T), kPieces = kPrGroup / (kPrLanes * V);
+  const int lit = threadIdx.x % kPrLanes, group = blockIdx.y;
+  const int c0 = group * kPrGroup;
+  for (int64_t base = (int64_t)blockIdx.x * kPrTeams; base < a.rows; base += (int64_t)gridDim.x * kPrTeams) {
+    const int64_t row = base + threadIdx.x / kPrLanes;
+    const bool live = row < a.rows;                      // dead teams stay: the moves need whole waves
+    const T* const src = static_cast<const T*>(a.x) + (live ? row : 0) * a.ldx;
+    float v[kPieces][V];
+    RowPiece<T, V> raw[kPieces];
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) raw[p].load(src, c0 + (p * kPrLanes + lit) * V, a.cols);
+    unsigned top = 0;
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+      raw[p].widen(v[p]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const unsigned m = __float_as_uint(v[p][j]) & 0x7fffffffu;
+        top = m > top ? m : top;
+      }
+    }
+    top = moved_max<0xB1>(top);                          // quad_perm [1,0,3,2]
+    top = moved_max<0x4E>(top);                          // quad_perm [2,3,0,1]
+    top = moved_max<0x141>(top);                         // row_half_mirror
+    const int b = exponent_byte<FMT>(top);
+    const float inv = __uint_as_float((unsigned)(254 - b) << 23);
+    if (!live) continue;
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+      const int c = c0 + (p * kPrLanes + lit) * V;
+      if (c >= a.pitch) continue;
+      uint8_t* const dst = a.codes + row * a.pitch + c;
+      unsigned w[V / 4];
+#pragma unroll
+      for (int q = 0; q < V / 4; ++q) w[q] = b == kPrNotFinite ? 0u : encode4<FMT>(&v[p][4 * q], inv);
+      if constexpr (V == 4) {
+        *reinterpret_cast<unsigned*>(dst) = w[0];
+      } else {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+      }
+    }
+    if (lit == 0) a.exps[row * a.groups + group] = (uint8_t)b;
+  }
+}
+
+template <typename T, int FMT> __global__ __launch_bounds__(kPrThreads) void unpack_rows_kernel(PackArgs a) {
+  constexpr int V = 16 / sizeof(T), kPieces = kPrGroup / (kPrLanes * V);
+  const int lit = threadIdx.x % kPrLanes, group = blockIdx.y;
+  const int c0 = group * kPrGroup;
+  for (int64_t row = (int64_t)blockIdx.x * kPrTeams + threadIdx.x / kPrLanes; row < a.rows;
+       row += (int64_t)gridDim.x * kPrTeams) {
+    const uint8_t* const src = a.codes + row * a.pitch;
+    unsigned w[kPieces][V / 4];
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+      const int c = c0 + (p * kPrLanes + lit) * V;
+#pragma unroll
+      for (int q = 0; q < V / 4; ++q) w[p][q] = 0;
+      if (c < a.pitch) {
+        if constexpr (V == 4) {
+          w[p][0] = *reinterpret_cast<const unsigned*>(src + c);
+        } else {
+          const uint2 t = *reinterpret_cast<const uint2*>(src + c);
+          w[p][0] = t.x; w[p][1] = t.y;
+        }
+      }
+    }
+    const float scale = packed_scale(a.exps[row * a.groups + group]);
+    T* const dst = static_cast<T*>(a.out) + row * a.cols;
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+      float v[V];
+#pragma unroll
+      for (int q = 0; q < V / 4; ++q) decode4<FMT>(w[p][q], scale, &v[4 * q]);
+      RowPiece<T, V> o;
+      o.narrow(v);
+      o.store(dst, c0 + (p * kPrLanes + lit) * V, a.cols);
+    }
+  }
+}
+
+int pack_check(int type, int fmt, int64_t rows, int cols) {
+  CXG_REQUIRE(rows >= 0 && cols >= 1, CXG_ERR_ARG, "bad rows/cols");
+  CXG_REQUIRE(value_type_ok(type), CXG_ERR_ARG, "unknown value type");
+  CXG_REQUIRE(fmt == CXG_PACK_INT8 || fmt == CXG_PACK_E4M3, CXG_ERR_ARG, "unknown 8-bit format");
+  CXG_REQUIRE(cols <= kPrMaxCols, CXG_ERR_UNSUPPORTED, "rows of more than %d columns", kPrMaxCols);
+  return CXG_OK;
+}
+
+dim3 pack_grid(int64_t rows, int groups) {
+  int64_t x = ceil_div(rows, (int64_t)kPrTeams);
+  const int64_t most = groups >= 64 ? 256 : 16384 / groups;      // rows per block beyond that: a loop
+  return dim3((unsigned)(x < most ? x : most), (unsigned)groups);
+}
+
+#define CXG_PR_LAUNCH(KERNEL, name)                                                                        \
+  do {                                                                                                     \
+    const dim3 grid = pack_grid(rows, a.groups), block(kPrThreads);                                        \
+    const bool i8 = fmt == CXG_PACK_INT8;                                                                  \
+    if (type == CXG_F32) {                                                                                 \
+      if (i8) hipLaunchKernelGGL((KERNEL<float, CXG_PACK_INT8>), grid, block, 0, st, a);                   \
+      else hipLaunchKernelGGL((KERNEL<float, CXG_PACK_E4M3>), grid, block, 0, st, a);                      \
+    } else if (type == CXG_BF16) {                                                                         \
+      if (i8) hipLaunchKernelGGL((KERNEL<bf16_t, CXG_PACK_INT8>), grid, block, 0, st, a);                  \
+      else hipLaunchKernelGGL((KERNEL<bf16_t, CXG_PACK_E4M3>), grid, block, 0, st, a);                     \
+    } else {                                                                                               \
+      if (i8) hipLaunchKernelGGL((KERNEL<f16_t, CXG_PACK_INT8>), grid, block, 0, st, a);                   \
+      else hipLaunchKernelGGL((KERNEL<f16_t, CXG_PACK_E4M3>), grid, block, 0, st, a);                      \
+    }                                                                                                      \
+    CXG_LAUNCH_CHECK(name);                                                                                \
+  } while (0)
+
+}  // namespace
+}  // namespace cxg
+
+extern "C" {
+
+int cxg_packed_pitch(int cols) { return cols < 1 ? 0 : cxg::packed_pitch(cols); }
+int cxg_packed_groups(int cols) { return cols < 1 ? 0 : cxg::packed_groups(cols); }
+
+int cxg_pack_rows(const void* x, int64_t ldx, int type, int fmt, int64_t rows, int cols, uint8_t* codes, uint8_t* exps,
+                  void* stream) {
+  using namespace cxg;
+  const int bad = pack_check(type, fmt, rows, cols);
+  if (bad) return bad;
+  if (rows == 0) return CXG_OK;
+  CXG_REQUIRE(x && codes && exps, CXG_ERR_ARG, "null x/codes/exps");
+  CXG_REQUIRE(ldx >= 0, CXG_ERR_ARG, "negative row stride");
+  CXG_REQUIRE(((uintptr_t)codes & 15) == 0, CXG_ERR_ARG, "codes must be 16-byte aligned");
+  CXG_REQUIRE(((uintptr_t)x & (value_bytes(type) - 1)) == 0, CXG_ERR_ARG, "x is not aligned to its values");
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  PackArgs a{x, ldx, codes, exps, nullptr, rows, cols, packed_pitch(cols), packed_groups(cols)};
+  CXG_PR_LAUNCH(pack_rows_kernel, "pack_rows_kernel");
+  return CXG_OK;
+}
+
+int cxg_unpack_rows(const uint8_t* codes, const uint8_t* exps, int fmt, int64_t rows, int cols, void* out, int type,
+                    void* stream) {
+  using namespace cxg;
+  const int bad = pack_check(type, fmt, rows, cols);
+  if (bad) return bad;
+  if (rows == 0) return CXG_OK;
+  CXG_REQUIRE(codes && exps && out, CXG_ERR_ARG, "null codes/exps/out");
+  CXG_REQUIRE(((uintptr_t)codes & 15) == 0, CXG_ERR_ARG, "codes must be 16-byte aligned");
+  CXG_REQUIRE(((uintptr_t)out & (value_bytes(type) - 1)) == 0, CXG_ERR_ARG, "out is not aligned to its values");
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  PackArgs a{nullptr, 0, const_cast<uint8_t*>(codes), const_cast<uint8_t*>(exps), out, rows, cols, packed_pitch(cols),
+             packed_groups(cols)};
+  CXG_PR_LAUNCH(unpack_rows_kernel, "unpack_rows_kernel");
+  return CXG_OK;
+}
+
+}  // extern "C"

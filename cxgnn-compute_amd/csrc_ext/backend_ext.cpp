@@ -1157,6 +1157,86 @@ std::tuple<OptTensor, OptTensor> residual_norm(const Tensor& x, const OptTensor&
   return std::make_tuple(r, y);
 }
 
+// ---------------------------------------------------------------------------------------------
+// rows held in 8 bits and the weight gradient that reads them (cxg_pack_rows, cxg_unpack_rows,
+// cxg_packed_wgrad; no counterpart in the reference)
+// ---------------------------------------------------------------------------------------------
+void* ptr_or_null_mut(const Tensor& t) { return t.defined() && t.numel() > 0 ? t.data_ptr() : nullptr; }
+// a map of no entries is a map all the same
+const void* map_ptr(const OptTensor& t) { return t.has_value() ? t->data_ptr() : nullptr; }
+std::string fmt_cols(int64_t cols) { return fmt("rows of %lld columns cannot be held in 8 bits", (long long)cols); }
+
+std::tuple<Tensor, Tensor> pack_rows(const Tensor& x_in, int64_t fmt) {
+  const Tensor x = rows_of(x_in, "x");
+  const int64_t rows = x.size(0), cols = x.size(1);
+  if (cols < 1 || cols > INT32_MAX) bad(fmt_cols(cols));
+  const auto bytes = x.options().dtype(at::kByte).requires_grad(false);
+  Tensor codes = torch::empty({rows, (int64_t)cxg_packed_pitch((int)cols)}, bytes);
+  Tensor exps = torch::empty({rows, (int64_t)cxg_packed_groups((int)cols)}, bytes);
+  c10::DeviceGuard guard(x.device());
+  check(cxg_pack_rows(ptr_or_null(x), x.stride(0), value_type(x, "x"), (int)fmt, rows, (int)cols, (uint8_t*)ptr_or_null_mut(codes),
+                      (uint8_t*)ptr_or_null_mut(exps), stream_of(x)));
+  return std::make_tuple(codes, exps);
+}
+
+// The codes and exponent bytes of rows of `cols` columns.
+void req_packed(const Tensor& codes, const Tensor& exps, int64_t cols) {
+  req(codes, "codes", at::kByte, {2});
+  req(exps, "exps", at::kByte, {2});
+  if (codes.device() != exps.device()) bad("codes and exps are on different devices");
+  if (cols < 1 || cols > INT32_MAX) bad(fmt_cols(cols));
+  if (codes.size(1) != cxg_packed_pitch((int)cols) || exps.size(1) != cxg_packed_groups((int)cols) || codes.size(0) != exps.size(0))
+    bad(fmt("rows of %lld columns have codes [n, %d] and exps [n, %d]", (long long)cols, cxg_packed_pitch((int)cols),
+            cxg_packed_groups((int)cols)));
+}
+
+Tensor unpack_rows(const Tensor& codes, const Tensor& exps, int64_t cols, int64_t fmt, const py::object& dtype) {
+  req_packed(codes, exps, cols);
+  Tensor out = torch::empty({codes.size(0), cols}, codes.options().dtype(torch::python::detail::py_object_to_dtype(dtype)));
+  c10::DeviceGuard guard(codes.device());
+  check(cxg_unpack_rows((const uint8_t*)ptr_or_null(codes), (const uint8_t*)ptr_or_null(exps), (int)fmt, codes.size(0), (int)cols,
+                        ptr_or_null_mut(out), value_type(out, "the unpacked rows"), stream_of(codes)));
+  return out;
+}
+
+// [R, K, N]; seg missing: one segment of all rows
+Tensor packed_wgrad(const Tensor& codes, const Tensor& exps, int64_t cols, int64_t fmt_id, const Tensor& g_in, const OptTensor& seg,
+                    const OptTensor& src, const OptTensor& dst) {
+  req_packed(codes, exps, cols);
+  const Tensor g = rows_of(g_in, "g");
+  same_device(g, codes, "g");
+  if (g.size(1) < 1 || g.size(1) > INT32_MAX) bad("g has no columns, or too many");
+  int64_t rows = -1, segs = 1;
+  for (const auto* map : {&src, &dst}) {
+    if (!map->has_value()) continue;
+    req(**map, "a row map", at::kLong, {1});
+    same_device(**map, codes, "a row map");
+    if (rows >= 0 && rows != (*map)->size(0)) bad("src_idx and dst_idx differ in length");
+    rows = (*map)->size(0);
+  }
+  if (rows < 0) {
+    if (codes.size(0) != g.size(0)) bad(fmt("%lld packed rows, %lld rows of g", (long long)codes.size(0), (long long)g.size(0)));
+    rows = g.size(0);
+  } else if ((!src.has_value() && codes.size(0) < rows) || (!dst.has_value() && g.size(0) < rows)) {
+    bad("fewer rows than the row map has entries");
+  }
+  if (seg.has_value()) {
+    req(*seg, "seg_ptr", at::kLong, {1});
+    same_device(*seg, codes, "seg_ptr");
+    segs = seg->size(0) - 1;
+    if (segs < 1) bad("seg_ptr needs at least two entries");
+  }
+  Tensor gw = torch::empty({segs, cols, g.size(1)}, codes.options().dtype(at::kFloat));
+  const int K = (int)cols, N = (int)g.size(1), R = (int)segs;
+  Tensor ws = workspace(cxg_packed_wgrad_workspace_bytes(rows, K, N, R), codes);
+  c10::DeviceGuard guard(codes.device());
+  check(cxg_packed_wgrad((const uint8_t*)ptr_or_null(codes), (const uint8_t*)ptr_or_null(exps), (int)fmt_id, codes.size(0),
+                         ptr_or_null(g), g.stride(0), value_type(g, "g"), g.size(0), (const int64_t*)map_ptr(src),
+                         (const int64_t*)map_ptr(dst), (const int64_t*)map_ptr(seg), rows, K, N, R, (float*)gw.data_ptr(),
+                         ws.data_ptr(), (size_t)ws.numel(), stream_of(codes)));
+  return gw;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1178,6 +1258,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("val") = py::none(), py::arg("val_perm") = py::none(), py::arg("out") = py::none(),
         py::arg("accumulate") = false, py::arg("bias") = py::none());
   m.def("head_sum", &head_sum);
+  m.def("pack_rows", &pack_rows, py::arg("x"), py::arg("fmt"));
+  m.def("unpack_rows", &unpack_rows, py::arg("codes"), py::arg("exps"), py::arg("cols"), py::arg("fmt"), py::arg("dtype"));
+  m.def("packed_wgrad", &packed_wgrad, py::arg("codes"), py::arg("exps"), py::arg("cols"), py::arg("fmt"), py::arg("g"),
+        py::arg("seg_ptr") = py::none(), py::arg("src_idx") = py::none(), py::arg("dst_idx") = py::none());
   m.def("residual_norm", &residual_norm, py::arg("x"), py::arg("f"), py::arg("gate"), py::arg("post"), py::arg("post_weight"),
         py::arg("post_bias"), py::arg("pre"), py::arg("pre_weight"), py::arg("pre_bias"), py::arg("res_scale"),
         py::arg("branch_scale"), py::arg("eps"));

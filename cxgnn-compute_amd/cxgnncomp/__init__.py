@@ -7,7 +7,7 @@ trainer and dataset loading of the reference need dgl / PyG / cxgnndl and are no
 this package.
 """
 from .graph_conv import (MyGATConv, MyGCNConv, MySageConv, MyGINConv, MyRGCNConv, RGCNOP, RGCNOP2,
-                         RGCNOP3, RGCNOP_sorted, AggrOP, AggrDirectedOP, SeastarRGCNOP, run_rgcn4)
+                         RGCNOP3, RGCNOP_sorted, AggrOP, AggrDirectedOP, SeastarRGCNOP, run_rgcn4, linear)
 from cxgnncomp_backend import (edge_attention, sage_sum_forward_edge_value, gather, sage_sum_forward,
                                aggr_rel, sage_mean_forward, aggr_rel_direct, rel_schedule, target_aggr)
 from .codegen import *  # noqa: F401,F403
@@ -22,6 +22,7 @@ from .util import global_tuner
 from .graph_kernel import SpMMValOP
 from .batchnorm import BatchNorm1d
 from .residual import ResidualNorm, residual_norm
+from .packed import PackedRows, pack_rows, packed_weight_grad
 from .model import (GNN, SAGE, GCN, GIN, GAT, RGCN, get_model, get_conv_from_str, get_model_from_str,
                     graph_type_dict, model_dict)
 from . import synthetic  # noqa: F401

@@ -785,6 +785,47 @@ int cxg_residual_norm_bwd(const void* x, int64_t ldx, const void* f, int64_t ldf
                           float* dpost_w, float* dpost_b, float* dpre_w, float* dpre_b,
                           void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------- */
+/* Rows held in 8 bits (no counterpart in the reference): what a layer keeps of */
+/* its input for the backward pass, and the weight gradient that reads it      */
+/* ------------------------------------------------------------------------- */
+
+#define CXG_PACK_INT8 0
+#define CXG_PACK_E4M3 1   /* float8 e4m3fn */
+
+/*
+ * Codes and scales of the rows of x [rows, cols] (fp32 / bf16 / fp16, row stride ldx in values).  128
+ * consecutive columns of a row share a scale 2^(b - 127); code = x / scale rounded to the nearest,
+ * ties to even; b is the smallest byte (at least 16) with which the largest magnitude fits: 127 after
+ * rounding (int8) or 448 (e4m3).  A group with an infinity or NaN has b = 255, codes 0, and reads back
+ * as NaN.  codes is [rows][cxg_packed_pitch(cols)] (columns rounded up to 16, zeros behind the last;
+ * 16-byte aligned), exps [rows][cxg_packed_groups(cols)].  Unpacking is exact in fp32 and bf16 (in
+ * fp16 it rounds) and writes contiguous rows.
+ */
+int cxg_packed_pitch(int cols);
+int cxg_packed_groups(int cols);
+int cxg_pack_rows(const void* x, int64_t ldx, int type, int fmt, int64_t rows, int cols,
+                  uint8_t* codes, uint8_t* exps, void* stream);
+int cxg_unpack_rows(const uint8_t* codes, const uint8_t* exps, int fmt, int64_t rows, int cols,
+                    void* out, int type, void* stream);
+
+/*
+ * Weight gradient from rows held in 8 bits: gw[r] (K x N, fp32, overwritten) = sum over the rows i of
+ * segment r of A[src(i), :]^T (x) G[dst(i), :]; segments without rows give zeros.  A: `codes` and
+ * `exps` as above with a_rows rows of K columns.  G: g_rows rows of N values of g_type, row stride ldg
+ * (aligned to its values).  src(i) = src_idx ? src_idx[i] : i, dst likewise; seg_ptr [R + 1] as in
+ * cxg_typed_gemm_f32, NULL for one segment of all M rows (R = 1).  A row whose src or dst lies outside
+ * its matrix is left out.  code * scale is a bf16 number and multiplies as it is; G goes in as one
+ * (bf16), two (fp16) or three (fp32) bf16 parts that add up to it exactly, accumulation is fp32.
+ * Partial sums over row chunks are added in a fixed order: results repeat bit for bit.  The workspace
+ * is 256-byte aligned.
+ */
+size_t cxg_packed_wgrad_workspace_bytes(int64_t M, int K, int N, int R);
+int cxg_packed_wgrad(const uint8_t* codes, const uint8_t* exps, int fmt, int64_t a_rows, const void* g,
+                     int64_t ldg, int g_type, int64_t g_rows, const int64_t* src_idx,
+                     const int64_t* dst_idx, const int64_t* seg_ptr, int64_t M, int K, int N, int R,
+                     float* gw, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
