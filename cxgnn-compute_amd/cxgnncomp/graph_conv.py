@@ -10,6 +10,7 @@ import math
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 from torch.nn import Parameter
 
 import cxgnncomp_backend
@@ -19,6 +20,7 @@ from cxgnncomp_backend import (aggr_rel, aggr_rgcn_direct_func, edge_attention, 
                                selective_aggr, selective_aggr_bwd)
 
 from .graph_kernel import SpMMValOP
+from .packed import PackedRows, check_format, pack_rows, packed_weight_grad
 from .timer import TimerOP
 from .typed_linear import (TypedLinearE2EOP, TypedLinearS2DAggrMMOP, TypedLinearS2DMMAggrOP,
                            TypedLinearS2DPushOP, TypedLinearS2DSort)
@@ -179,8 +181,11 @@ def run_rgcn4(x, ptr, idx, edge_types, linear, num_center, num_edge, preproccess
 
 class MySageConv(torch.nn.Module):
 
-    def __init__(self, in_channels, hidden_channels, root_weight=True, bias=True):
+    def __init__(self, in_channels, hidden_channels, root_weight=True, bias=True, checkpoint=None):
+        """``checkpoint`` (not upstream) "int8" or "e4m3": the inputs of the layer's linear maps are kept
+        for the backward pass in 8 bits per value (``linear``)."""
         super().__init__()
+        self.checkpoint = check_format(checkpoint)
         self.in_channels = in_channels
         self.hidden_channels = hidden_channels
         self.root_weight = root_weight
@@ -195,22 +200,26 @@ class MySageConv(torch.nn.Module):
             self.lin_r.reset_parameters()
 
     def forward(self, x, ptr, idx, num_node):
-        if x.is_cuda and x.dim() == 2:
+        if x.is_cuda and x.dim() == 2 and self.checkpoint is None:
             return SageLayerOP.apply(x, self.lin_l.weight, self.lin_l.bias,
                                      self.lin_r.weight if self.root_weight else None, ptr, idx, num_node)
         if self.in_channels > self.hidden_channels:
-            out = sage_mean_forward(linear(x, self.lin_l.weight, self.lin_l.bias), ptr, idx, num_node)
+            out = sage_mean_forward(linear(x, self.lin_l.weight, self.lin_l.bias, checkpoint=self.checkpoint), ptr, idx, num_node)
         else:
-            out = linear(sage_mean_forward(x, ptr, idx, num_node), self.lin_l.weight, self.lin_l.bias)
+            out = linear(sage_mean_forward(x, ptr, idx, num_node), self.lin_l.weight, self.lin_l.bias,
+                         checkpoint=self.checkpoint)
         if self.root_weight:
-            out = linear(x[:num_node] if num_node != 0 else x, self.lin_r.weight, addend=out)
+            out = linear(x[:num_node] if num_node != 0 else x, self.lin_r.weight, addend=out, checkpoint=self.checkpoint)
         return out
 
 
 class MyGINConv(torch.nn.Module):
 
-    def __init__(self, in_channels, hidden_channels):
+    def __init__(self, in_channels, hidden_channels, checkpoint=None):
+        """``checkpoint`` (not upstream) "int8" or "e4m3": the input of the layer's linear map is kept for
+        the backward pass in 8 bits per value (``linear``)."""
         super().__init__()
+        self.checkpoint = check_format(checkpoint)
         self.in_channels = in_channels
         self.hidden_channels = hidden_channels
         self.nn = torch.nn.Linear(in_channels, hidden_channels, bias=False)
@@ -224,7 +233,7 @@ class MyGINConv(torch.nn.Module):
 
     def forward(self, x, ptr, idx, num_node):
         out = sage_mean_forward(x, ptr, idx, num_node)
-        return linear(out + (1 + self.eps) * x[:num_node], self.nn.weight)
+        return linear(out + (1 + self.eps) * x[:num_node], self.nn.weight, checkpoint=self.checkpoint)
 
 
 class MyRGCNConv(torch.nn.Module):
@@ -451,9 +460,59 @@ class LinearOP(torch.autograd.Function):
         return tuple(grads[i] if need else None for i, need in enumerate(ctx.needs_input_grad))
 
 
-def linear(x, weight, bias=None, addend=None):
+class PackedLinearOP(torch.autograd.Function):
+    """``LinearOP`` whose input is kept for the backward pass in 8 bits (``pack_rows``) instead of as it
+    is: a quarter of the memory of fp32 rows, half of bf16.  Output, input gradient and bias gradient
+    are LinearOP's; the weight gradient is that of the rows the 8 bits stand for, multiplied from them
+    directly (``packed_weight_grad``)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, addend, fmt):
+        packed = pack_rows(x.reshape(-1, x.shape[-1]), fmt) if ctx.needs_input_grad[1] else None
+        ctx.fmt, ctx.shape = fmt, x.shape
+        ctx.save_for_backward(weight, *(() if packed is None else (packed.codes, packed.exps)))
+        return _linear_product(x, weight, bias, addend)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        weight, codes, exps = (ctx.saved_tensors + (None, None))[:3]
+        gx = gw = gb = None
+        if ctx.needs_input_grad[0]:
+            gx = _typed.dense_linear(g, weight) if g.dim() == 2 else None
+            if gx is None:
+                gx = g @ weight
+        if ctx.needs_input_grad[1]:
+            packed = PackedRows(codes, exps, ctx.shape[-1], ctx.fmt)
+            gw = packed_weight_grad(packed, g.reshape(-1, g.shape[-1]))[0].t().to(weight.dtype)
+        if ctx.needs_input_grad[2]:
+            gb = _bias_grad(g)
+        return gx, gw, gb, g if ctx.needs_input_grad[3] else None, None
+
+
+def _linear_product(x, weight, bias, addend):
+    out = _typed.dense_linear(x, weight.t(), bias, addend)
+    if out is not None:
+        return out
+    if addend is None:
+        return F.linear(x, weight, bias)
+    out = torch.addmm(addend, x, weight.t())
+    return out if bias is None else out.add_(bias)
+
+
+def _bias_grad(g):
+    g = g.reshape(-1, g.shape[-1])
+    return _ops.column_sum(g.contiguous()) if g.dtype == torch.float32 else g.sum(dim=0)
+
+
+def linear(x, weight, bias=None, addend=None, checkpoint=None):
     """``F.linear(x, weight, bias)``, plus ``addend`` where given, for the conv layers; CUDA
-    tensors take LinearOP."""
+    tensors take LinearOP.  ``checkpoint`` "int8" or "e4m3": what the weight gradient needs of x is
+    kept in 8 bits per value (PackedLinearOP; CUDA tensors, float32 / bfloat16 / float16)."""
+    if check_format(checkpoint) is not None and x.is_cuda:
+        if addend is not None and x.dim() != 2:
+            raise ValueError("an addend goes with x [N, C]")
+        return PackedLinearOP.apply(x, weight, bias, addend, checkpoint)
     if not x.is_cuda or (addend is not None and x.dim() != 2):
         out = F.linear(x, weight, bias)
         return out if addend is None else addend + out
@@ -781,8 +840,11 @@ class MyGATConv(torch.nn.Module):
 
 class MyGCNConv(torch.nn.Module):
 
-    def __init__(self, in_channels, out_channels, normalize=False, bias=True):
+    def __init__(self, in_channels, out_channels, normalize=False, bias=True, checkpoint=None):
+        """``checkpoint`` (not upstream) "int8" or "e4m3": the input of the layer's linear map is kept for
+        the backward pass in 8 bits per value (``linear``)."""
         super().__init__()
+        self.checkpoint = check_format(checkpoint)
         self.in_channels = in_channels
         self.out_channels = out_channels
         self.normalize = normalize
@@ -807,7 +869,7 @@ class MyGCNConv(torch.nn.Module):
     def forward(self, x, ptr, idx, num_node):
         x = TimerOP.apply(x, "linear", True)
         mm_before = self.in_channels > self.out_channels
-        out = linear(x, self.lin.weight) if mm_before else x
+        out = linear(x, self.lin.weight, checkpoint=self.checkpoint) if mm_before else x
         out = TimerOP.apply(out, "linear", False)
         if self.normalize:
             out = TimerOP.apply(out, "aggregation", True)
@@ -819,5 +881,5 @@ class MyGCNConv(torch.nn.Module):
         else:
             out = AggrOP.apply(out, ptr, idx, num_node)
         if not mm_before:
-            return linear(out, self.lin.weight, self.bias)
+            return linear(out, self.lin.weight, self.bias, checkpoint=self.checkpoint)
         return out + self.bias if self.bias is not None else out

@@ -9,6 +9,13 @@
 
 Between layers: BatchNorm1d, ReLU, dropout; the output is ``log_softmax``.  The DGL /
 PyG graph types of the reference need those packages and raise here.
+
+Two options that upstream does not have, for deep stacks on large graphs:
+  * ``residual`` "layer" or "rms": instead of batch norm the layers are the blocks of a residual
+    stream, r = r + gate * post(relu(layer(dropout(pre(r))))) with layer or rms norms of the rows
+    (``ResidualNorm``); the first layer opens the stream, the last reads it;
+  * ``checkpoint`` "int8" or "e4m3" (SAGE, GCN, GIN): the inputs of the layers' linear maps are kept
+    for the backward pass in 8 bits per value.
 """
 import torch
 import torch.nn.functional as F
@@ -17,6 +24,8 @@ import cxgnncomp_backend
 
 from .batchnorm import BatchNorm1d
 from .graph_conv import MyGATConv, MyGCNConv, MyGINConv, MyRGCNConv, MySageConv
+from .packed import check_format
+from .residual import ResidualNorm
 
 
 def _need_csr(graph_type):
@@ -27,17 +36,28 @@ def _need_csr(graph_type):
 
 class GNN(torch.nn.Module):
 
+    packs_inputs = False              # whether the layers take ``checkpoint``
+
     def __init__(self, in_channels, hidden_channels, out_channels, num_layer, dropout, graph_type,
-                 config=None, **kwargs):
+                 config=None, residual=None, checkpoint=None, **kwargs):
         super().__init__()
         _need_csr(graph_type)
+        if residual not in (None, "layer", "rms"):
+            raise ValueError("residual must be None, 'layer' or 'rms', got %r" % (residual, ))
+        if check_format(checkpoint) is not None and not self.packs_inputs:
+            raise ValueError("%s keeps no input of a linear map that could be held in 8 bits" % type(self).__name__)
+        self.residual, self.checkpoint = residual, checkpoint
         self.in_channels = in_channels
         self.hidden_channels = hidden_channels
         self.out_channels = out_channels
         self.graph_type = graph_type
         self.num_layer = num_layer
         self.dropout = dropout
-        self.bns = torch.nn.ModuleList(BatchNorm1d(hidden_channels) for _ in range(num_layer - 1))
+        self.bns = torch.nn.ModuleList(BatchNorm1d(hidden_channels) for _ in range(num_layer - 1 if residual is None else 0))
+        if residual is not None:
+            self.norms = torch.nn.ModuleList(
+                ResidualNorm(hidden_channels, post=residual if i else None, pre=residual, gate="channel" if i else None)
+                for i in range(num_layer - 1))
         self.init_convs(**kwargs)
 
     def init_convs(self, **kwargs):
@@ -52,7 +72,7 @@ class GNN(torch.nn.Module):
         raise NotImplementedError
 
     def reset_parameters(self):
-        for m in list(self.convs) + list(self.bns):
+        for m in list(self.convs) + list(self.bns) + list(self.norms if self.residual is not None else ()):
             m.reset_parameters()
 
     # rows / edges layer i works on
@@ -80,11 +100,28 @@ class GNN(torch.nn.Module):
             cxgnncomp_backend._ops.note_edge_counts(batch.ptr, batch.idx, batch.num_node_in_layer[:-1],
                                                     batch.num_edge_in_layer)
         last = self.num_layer - 1
+        if self.residual is not None:
+            return self._forward_residual(x, batch, skip_first)
         for i, conv in enumerate(self.convs):
             if not (skip_first and i == 0 and i != last):
                 x = self.layer(conv, x, batch, i)
             if i != last:
                 x = self._between(x, i)
+        return x.log_softmax(dim=-1)
+
+    def _forward_residual(self, x, batch, skip_first):
+        last, stream = self.num_layer - 1, None
+        for i, conv in enumerate(self.convs):
+            if not (skip_first and i == 0 and i != last):
+                x = self.layer(conv, x, batch, i)
+            if i == last:
+                break
+            x = F.relu(x)
+            if i == 0:
+                stream, x = self.norms[0].enter(x)
+            else:
+                stream, x = self.norms[i](stream[:x.shape[0]], x)      # a layer's rows are a prefix of its input's
+            x = F.dropout(x, p=self.dropout, training=self.training)
         return x.log_softmax(dim=-1)
 
     def forward(self, input, skip_first=False):
@@ -93,21 +130,24 @@ class GNN(torch.nn.Module):
 
 
 class SAGE(GNN):
+    packs_inputs = True
 
     def init_conv(self, in_channels, out_channels, **kwargs):
-        return MySageConv(in_channels, out_channels)
+        return MySageConv(in_channels, out_channels, checkpoint=self.checkpoint)
 
 
 class GCN(GNN):
+    packs_inputs = True
 
     def init_conv(self, in_channels, out_channels, **kwargs):
-        return MyGCNConv(in_channels, out_channels)
+        return MyGCNConv(in_channels, out_channels, checkpoint=self.checkpoint)
 
 
 class GIN(GNN):
+    packs_inputs = True
 
     def init_conv(self, in_channels, out_channels, **kwargs):
-        return MyGINConv(in_channels, out_channels)
+        return MyGINConv(in_channels, out_channels, checkpoint=self.checkpoint)
 
 
 class GAT(GNN):
@@ -197,19 +237,20 @@ def get_model(config):
     """Model from a training configuration (cxgnncomp/model.py:362-399): reads
     ``dl.dataset.{feature_dim, num_classes, name}``, ``dl.sampler.train.num_layer``,
     ``train.type`` (cxg / dgl / pyg) and ``train.model.{type, hidden_dim, dropout, heads, concat,
-    num_rel}``.  The dgl / pyg graph types raise NotImplementedError."""
+    num_rel}``, and ``residual`` / ``checkpoint`` where given.  The dgl / pyg graph types raise NotImplementedError."""
     dataset = config.dl.dataset
     spec = config.train.model
     kind = str(_item(spec, "type")).lower()
     graph_type = graph_type_dict[str(config.train.type).lower()]
     args = (_item(dataset, "feature_dim"), _item(spec, "hidden_dim"), _item(dataset, "num_classes"),
             config.dl.sampler.train.num_layer, _item(spec, "dropout"), graph_type, config)
+    options = dict(residual=_item(spec, "residual"), checkpoint=_item(spec, "checkpoint"))
     if "gat" in kind:
-        return model_dict[kind](*args, heads=_item(spec, "heads", 1), concat=_item(spec, "concat", False))
+        return model_dict[kind](*args, **options, heads=_item(spec, "heads", 1), concat=_item(spec, "concat", False))
     if "rgcn" in kind:
-        return model_dict[kind](*args, num_rel=int(_item(spec, "num_rel")),
+        return model_dict[kind](*args, **options, num_rel=int(_item(spec, "num_rel")),
                                 dataset_name=str(_item(dataset, "name")).lower())
-    return model_dict[kind](*args)
+    return model_dict[kind](*args, **options)
 
 
 def get_conv_from_str(model_str, infeat, outfeat, num_head=-1, num_rel=-1):
@@ -227,11 +268,11 @@ def get_conv_from_str(model_str, infeat, outfeat, num_head=-1, num_rel=-1):
 
 
 def get_model_from_str(mtype, infeat, hiddenfeat, outfeat, graph_type, num_layer, num_head=-1, num_rel=-1,
-                       dataset=None, dropout=0.5):
-    """One layer stack by name (cxgnncomp/model.py:417-467).  ``LSTM`` (the neighbour-LSTM
+                       dataset=None, dropout=0.5, residual=None, checkpoint=None):
+    """One layer stack by name (cxgnncomp/model.py:417-467; ``residual`` and ``checkpoint`` as for GNN).  ``LSTM`` (the neighbour-LSTM
     aggregator) is outside this package."""
     mtype = mtype.upper()
-    common = dict(dropout=dropout, graph_type=graph_type, config=None)
+    common = dict(dropout=dropout, graph_type=graph_type, config=None, residual=residual, checkpoint=checkpoint)
     if mtype == "GCN":
         return GCN(infeat, hiddenfeat, outfeat, num_layer, **common)
     if mtype == "GAT":

@@ -16,6 +16,7 @@ import cxgnncomp_backend
 from cxgnncomp_backend import _ops, _typed
 
 from .codegen.typed_matmul import typed_matmul
+from .packed import PackedRows, check_format, pack_rows, packed_weight_grad
 
 
 def TypedLinearNaiveS2D(x, weights, types, src, dst, num_center, num_edge):
@@ -54,7 +55,9 @@ def _weight_grad(x_rows, g_rows, perm, seg, shape):
 
 
 class TypedLinearE2EOP(torch.autograd.Function):
-    """out[i] = x[i] @ weights[types[i]] for edge-level x [E, K]."""
+    """out[i] = x[i] @ weights[types[i]] for edge-level x [E, K].  ``checkpoint`` "int8" or "e4m3"
+    (not upstream): x is kept for the weight gradient in 8 bits per value (``pack_rows``), which
+    then is that of the rows the 8 bits stand for."""
 
     @staticmethod
     def preprocess(weights, types, thres=256):
@@ -72,7 +75,8 @@ class TypedLinearE2EOP(torch.autograd.Function):
         return [sorted_types, num_item, indices, count.cpu()]
 
     @staticmethod
-    def forward(ctx, x, weights, types, preprocessed=[], thres=256, count=None):
+    def forward(ctx, x, weights, types, preprocessed=[], thres=256, count=None, checkpoint=None):
+        check_format(checkpoint)
         if len(preprocessed) == 4:
             sorted_types, num_item, indices, count = preprocessed
         else:
@@ -82,13 +86,20 @@ class TypedLinearE2EOP(torch.autograd.Function):
         # padding rows carry indices >= num_item; typed_matmul drops them.  The real rows
         # are a permutation of 0..num_item-1, so every output row is written.
         output = typed_matmul(x, weights, sorted_types, num_item, indices, covers_output=True)
-        ctx.save_for_backward(x, weights, types, indices, sorted_types)
-        ctx.num_item = num_item
+        if checkpoint is None:
+            kept = (x, )
+        elif ctx.needs_input_grad[1]:
+            packed = pack_rows(x, checkpoint)
+            kept = (packed.codes, packed.exps)
+        else:
+            kept = ()
+        ctx.save_for_backward(weights, types, indices, sorted_types, *kept)
+        ctx.num_item, ctx.checkpoint = num_item, checkpoint
         return output[:num_item]
 
     @staticmethod
     def backward(ctx, grad_out):
-        x, weights, types, indices, sorted_types = ctx.saved_tensors
+        weights, types, indices, sorted_types, *kept = ctx.saved_tensors
         grad_out = grad_out.contiguous()
         grad_x = grad_w = None
         if ctx.needs_input_grad[0]:
@@ -96,8 +107,12 @@ class TypedLinearE2EOP(torch.autograd.Function):
             grad_x = typed_matmul(grad_out, wt, sorted_types, ctx.num_item, indices, covers_output=True)
         if ctx.needs_input_grad[1]:
             perm, seg = _typed.rel_segment(types.contiguous(), weights.shape[0])
-            grad_w = _weight_grad(x, grad_out, perm, seg, weights.shape)
-        return grad_x, grad_w, None, None, None, None
+            if ctx.checkpoint is None:
+                grad_w = _weight_grad(kept[0], grad_out, perm, seg, weights.shape)
+            else:
+                packed = PackedRows(kept[0], kept[1], weights.shape[1], ctx.checkpoint)
+                grad_w = packed_weight_grad(packed, grad_out, seg, src_idx=perm, dst_idx=perm)
+        return grad_x, grad_w, None, None, None, None, None
 
 
 class TypedLinearS2EOP(torch.autograd.Function):
