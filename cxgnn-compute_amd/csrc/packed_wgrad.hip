@@ -21,7 +21,8 @@
 // chunks of a segment in order: no atomics.
 //
 // Row numbers that come from maps are fetched by the first wave two steps ahead into a ring in LDS
-// and checked there; a row outside its matrix counts as no row.
+// and checked there; a row outside its matrix counts as no row.  Exponent bytes come through LDS too,
+// one load of the second wave per step.
 #include "packed_rows.hpp"
 
 namespace cxg {
@@ -33,11 +34,19 @@ typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 
 constexpr int kPwThreads = 256;
 constexpr int kPwXcds = 8;               // accelerator dies, one L2 each
-constexpr int kPwRows = 32;              // rows per step
-constexpr int kPwPitch = kPwRows + 8;    // LDS row pitch in bf16: 80 bytes
-constexpr int kPwTile = 128;
-constexpr int kPwBlocksPerCu = 3;
-static_assert(kPwTile == kPrGroup, "one scale per row and tile");
+constexpr int kPwTile = 128;             // columns of G of a tile, and of A per scale group
+constexpr int kPwFront = 8;              // columns in front of a tile of G: at least what a thread stages
+static_assert(kPwTile == kPrGroup, "one scale per row and 128 columns");
+
+// Shape of a block: KT columns of A, ROWS rows per step, BLOCKS of them per CU.
+template <int KT_, int ROWS_, int BLOCKS_> struct PwShape {
+  static constexpr int KT = KT_, ROWS = ROWS_, BLOCKS = BLOCKS_;
+  static constexpr int PITCH = ROWS + 8;                      // LDS pitch in bf16: 80 or 144 bytes
+  static constexpr int MG = ROWS / 4;                         // groups of four rows
+  static constexpr int CA = KT * ROWS / (4 * kPwThreads);     // columns of A / G that a thread stages
+  static constexpr int CG = kPwTile * ROWS / (4 * kPwThreads);
+  static constexpr int MI = KT / 64;                          // 32 x 32 blocks of a wave along K; two along N
+};
 
 struct PwArgs {
   const uint8_t* codes; const uint8_t* exps;
@@ -88,148 +97,236 @@ __device__ __forceinline__ unsigned bf16_pair(float x, float y) {
   return __builtin_bit_cast(unsigned, t);
 }
 
-template <int FMT, typename TG, bool MAPPED>
-__global__ __launch_bounds__(kPwThreads, kPwBlocksPerCu) void packed_wgrad_kernel(PwArgs a) {
+template <int FMT, typename TG, bool MAPPED, typename S, bool TINY>
+__global__ __launch_bounds__(kPwThreads, S::BLOCKS) void packed_wgrad_kernel(PwArgs a) {
   constexpr int NP = PwParts<TG>::value;
-  __shared__ __attribute__((aligned(16))) uint16_t s_a[kPwTile][kPwPitch];
-  __shared__ __attribute__((aligned(16))) uint16_t s_g[NP][kPwTile][kPwPitch];
-  __shared__ int64_t s_ids[MAPPED ? 3 : 1][2][kPwRows];
-  const int n_ct = (a.N + kPwTile - 1) / kPwTile, n_kt = (a.K + kPwTile - 1) / kPwTile, n_tile = n_ct * n_kt;
+  constexpr int ROWS = S::ROWS, MG = S::MG, CA = S::CA, CG = S::CG, MI = S::MI, PITCH = S::PITCH, NG = S::KT / kPrGroup;
+  __shared__ __attribute__((aligned(16))) uint16_t s_a[S::KT][PITCH];
+  __shared__ __attribute__((aligned(16))) uint16_t s_gp[NP][kPwFront + kPwTile][PITCH];   // kPwFront columns of slack in front
+  __shared__ __attribute__((aligned(16))) uint8_t s_exp[2][NG][ROWS];                     // exponent bytes of a step's rows
+  __shared__ int64_t s_off[MAPPED ? 3 : 1][3][MAPPED ? ROWS : 1];                         // ring: offsets of the rows of codes, exps, g
+  __shared__ unsigned long long s_live[3];                                                // and which of them are there
+  const int n_ct = (a.N + kPwTile - 1) / kPwTile, n_kt = (a.K + S::KT - 1) / S::KT, n_tile = n_ct * n_kt;
   const int64_t slot = blockIdx.x / kPwXcds;
   const int64_t chunk = (slot / n_tile) * kPwXcds + (blockIdx.x % kPwXcds);
-  const int kt = (int)((slot % n_tile) / n_ct);
-  const int n0 = (int)((slot % n_tile) % n_ct) * kPwTile, k0 = kt * kPwTile;
+  const int k0 = (int)((slot % n_tile) / n_ct) * S::KT;
+  const int n0 = (int)((slot % n_tile) % n_ct) * kPwTile;
   int64_t row0 = 0, row_end = 0;
   if (chunk >= a.chunks || !pw_locate(a, chunk, row0, row_end)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform_i32(tid >> 6);
-  const int steps = (int)((row_end - row0 + kPwRows - 1) / kPwRows);
+  const int steps = (int)((row_end - row0 + ROWS - 1) / ROWS);
+  const int last_rows = (int)(row_end - row0 - (int64_t)(steps - 1) * ROWS);
 
-  // staging: rows 4 mg .. 4 mg + 3 of a step, columns 4 c4 .. 4 c4 + 3 of the tile.  The low lane bits
-  // select the rows: the lanes the LDS serves together then write different banks.
-  const int mg = lane & 7, c4 = wave * 8 + (lane >> 3);
-  const bool a_col = k0 + 4 * c4 < a.pitch;
-  const uint8_t* const a_base = a.codes + k0 + 4 * c4;
-  const uint8_t* const e_base = a.exps + kt;
-  const TG* const g_base = static_cast<const TG*>(a.g);
-  unsigned code[4];
-  unsigned expo[4];
-  RowPiece<TG, 4> gv[4];
+  // staging: rows 4 mg .. 4 mg + 3 of a step, CA columns of A and CG of G.  The low lane bits select the
+  // rows: the lanes the LDS serves together then write different banks.
+  // All loads of the loop are unconditional, so that none waits for another: columns of A past the
+  // pitch read column k0, a piece of G that would pass N is moved back to end there (it then writes the
+  // columns it shares with its neighbour twice, the same values, and those in front of the tile into the
+  // slack), rows that are not there read row 0 and are cleared when they are staged.  What is staged
+  // for columns of A or G that do not exist only reaches rows and columns of gW that do not exist.
+  const int mg = lane % MG, cg = wave * (64 / MG) + lane / MG;
+  const int ka = k0 + CA * cg;
+  const uint8_t* const a_base = a.codes + (ka < a.pitch ? ka : k0);
+  int ng = n0 + CG * cg;
+  if (!TINY && ng + CG > a.N) ng = a.N - CG;                    // N >= CG
+  const int gcol = TINY ? kPwFront + CG * cg : kPwFront + ng - n0 < 0 ? 0 : kPwFront + ng - n0;
+  const TG* const g_base = static_cast<const TG*>(a.g) + (TINY ? 0 : ng);
+  // exponent bytes: lane of the second wave -> (group, row)
+  const int e_grp = (k0 / kPrGroup + lane / ROWS) < a.groups ? k0 / kPrGroup + lane / ROWS : a.groups - 1;
+  unsigned code[4][CA / 4];
+  TG gv[4][CG];
+  unsigned expo[(NG * ROWS + 63) / 64];
 
-  // MAPPED: lanes 0-31 of the first wave fetch the rows of A, lanes 32-63 those of G; a row that is
-  // missing in either matrix is -1 in both
-  auto fetch_ids = [&](int t) -> int64_t {
-    const int64_t at = row0 + (int64_t)t * kPwRows + (lane & 31);
-    int64_t id = -1;
-    if (at < row_end) {
-      const int64_t* const map = lane < 32 ? a.src : a.dst;
-      id = map ? map[at] : at;
-      if (id < 0 || id >= (lane < 32 ? a.a_rows : a.g_rows)) id = -1;
+  auto load_row = [&](int i, int64_t oa, int64_t og) {
+    typedef unsigned piece_t __attribute__((ext_vector_type(CA / 4)));
+    const piece_t w = *reinterpret_cast<const piece_t*>(a_base + oa);
+#pragma unroll
+    for (int j = 0; j < CA / 4; ++j) code[i][j] = w[j];
+    if constexpr (TINY) {
+#pragma unroll
+      for (int j = 0; j < CG; ++j) gv[i][j] = g_base[og + (ng + j < a.N ? ng + j : a.N - 1)];
+    } else {
+      constexpr int V = 16 / (int)sizeof(TG) < CG ? 16 / (int)sizeof(TG) : CG;
+#pragma unroll
+      for (int q = 0; q < CG / V; ++q) {
+        const auto p = *reinterpret_cast<const typename RowPiece<TG, V>::loose_t*>(g_base + og + q * V);
+#pragma unroll
+        for (int j = 0; j < V; ++j) gv[i][q * V + j] = p[j];
+      }
     }
-    const int other = __shfl_xor(id >= 0 ? 1 : 0, 32, CXG_WAVE);
-    return other ? id : -1;
   };
+  // MAPPED: lane r of the first wave loads the map entries of row r of step t (of the last row behind the
+  // end), and turns them into offsets a step later
+  const int64_t* const map_a = a.src ? a.src : a.dst;
+  const int64_t* const map_g = a.dst ? a.dst : a.src;
+  auto clamped = [&](int t) -> int64_t {
+    const int64_t at = row0 + (int64_t)t * ROWS + (lane & (ROWS - 1));
+    return at < row_end ? at : row_end - 1;
+  };
+  auto put = [&](int t, int64_t ia, int64_t ig) {
+    const int64_t at = row0 + (int64_t)t * ROWS + (lane & (ROWS - 1));
+    ia = a.src ? ia : at;
+    ig = a.dst ? ig : at;
+    const bool ok = at < row_end && ia >= 0 && ia < a.a_rows && ig >= 0 && ig < a.g_rows;
+    const unsigned long long live = __ballot(ok);
+    if (lane < ROWS) {
+      s_off[t % 3][0][lane] = ok ? ia * a.pitch : 0;
+      s_off[t % 3][1][lane] = ok ? ia * a.groups : 0;
+      s_off[t % 3][2][lane] = ok ? ig * a.ldg : 0;
+    }
+    if (lane == 0) s_live[t % 3] = live;
+  };
+  // rows of step t into registers; behind the last step the last one again
   auto load = [&](int t) {
+    t = t < steps ? t : steps - 1;
+    const int64_t first = row0 + (int64_t)t * ROWS;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      int64_t ia, ig;
       if constexpr (MAPPED) {
-        ia = s_ids[t % 3][0][4 * mg + i];
-        ig = s_ids[t % 3][1][4 * mg + i];
+        load_row(i, s_off[t % 3][0][4 * mg + i], s_off[t % 3][2][4 * mg + i]);
       } else {
-        ia = row0 + (int64_t)t * kPwRows + 4 * mg + i;
-        if (ia >= row_end) ia = -1;
-        ig = ia;
+        const int64_t r = first + 4 * mg + i < row_end ? first + 4 * mg + i : row0;
+        load_row(i, r * a.pitch, r * a.ldg);
       }
-      code[i] = 0;
-      expo[i] = 0;
+    }
+    if (wave == 1) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) gv[i].t[j] = (TG)0.f;
-      if (ia >= 0) {
-        if (a_col) code[i] = *reinterpret_cast<const unsigned*>(a_base + ia * a.pitch);
-        expo[i] = e_base[ia * a.groups];
-        gv[i].load(g_base + ig * a.ldg, n0 + 4 * c4, a.N);
+      for (int q = 0; q < (NG * ROWS + 63) / 64; ++q) {
+        const int row = lane & (ROWS - 1);
+        int64_t o;
+        if constexpr (MAPPED) o = s_off[t % 3][1][row];
+        else o = (first + row < row_end ? first + row : row0) * a.groups;
+        expo[q] = a.exps[o + (ROWS == 64 ? (e_grp + q < a.groups ? e_grp + q : a.groups - 1) : e_grp)];
       }
     }
   };
-  auto stage = [&]() {
-    float v[4][4];
+  auto put_exp = [&](int t) {
+    if (wave == 1) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) decode4<FMT>(code[i], packed_scale(expo[i]), v[i]);
+      for (int q = 0; q < (NG * ROWS + 63) / 64; ++q)
+        if (q * 64 + lane < NG * ROWS) s_exp[t & 1][ROWS == 64 ? q : lane / ROWS][lane & (ROWS - 1)] = (uint8_t)expo[q];
+    }
+  };
+  auto stage = [&](int t) {
+    unsigned exps = *reinterpret_cast<const unsigned*>(&s_exp[t & 1][NG == 1 ? 0 : CA * cg / kPrGroup][4 * mg]);
+    unsigned live;                                       // which of this thread's four rows are there
+    bool whole;
+    if constexpr (MAPPED) {
+      const unsigned long long m = s_live[t % 3];
+      live = (unsigned)(m >> (4 * mg)) & 15u;
+      whole = (ROWS == 64 ? m : m | 0xffffffff00000000ull) == ~0ull;
+    } else {
+      const int here = t + 1 < steps ? ROWS : last_rows;
+      whole = here == ROWS;
+      const int n = here - 4 * mg;
+      live = n >= 4 ? 15u : n <= 0 ? 0u : (1u << n) - 1u;
+    }
+    if (!whole) {
+      // a row that is not there is a row of zeros on both sides (0 times something not finite is NaN)
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      *reinterpret_cast<uint2*>(&s_a[4 * c4 + c][4 * mg]) = make_uint2(bf16_pair(v[0][c], v[1][c]), bf16_pair(v[2][c], v[3][c]));
+      for (int i = 0; i < 4; ++i) {
+        const bool on = (live >> i) & 1u;
+        exps &= on ? ~0u : ~(0xffu << (8 * i));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) gv[i].widen(v[i]);
+        for (int j = 0; j < CA / 4; ++j) code[i][j] = on ? code[i][j] : 0u;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      float x[4] = {v[0][c], v[1][c], v[2][c], v[3][c]};
+        for (int j = 0; j < CG; ++j) gv[i][j] = on ? gv[i][j] : (TG)0.f;
+      }
+    }
 #pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        const unsigned lo = bf16_pair(x[0], x[1]), hi = bf16_pair(x[2], x[3]);
-        *reinterpret_cast<uint2*>(&s_g[p][4 * c4 + c][4 * mg]) = make_uint2(lo, hi);
-        if (p + 1 < NP) {
-          x[0] -= __uint_as_float(lo << 16);
-          x[1] -= __uint_as_float(lo & 0xffff0000u);
-          x[2] -= __uint_as_float(hi << 16);
-          x[3] -= __uint_as_float(hi & 0xffff0000u);
+    for (int q = 0; q < CA / 4; ++q) {
+      float v[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) decode4<FMT>(code[i][q], packed_scale((exps >> (8 * i)) & 0xffu), v[i]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        *reinterpret_cast<uint2*>(&s_a[CA * cg + 4 * q + c][4 * mg]) =
+            make_uint2(bf16_pair(v[0][c], v[1][c]), bf16_pair(v[2][c], v[3][c]));
+    }
+#pragma unroll
+    for (int c = 0; c < CG; ++c) {
+      if constexpr (NP == 1) {
+        // bf16 values go through as they are
+        uint2 o;
+        o.x = (unsigned)__builtin_bit_cast(uint16_t, gv[0][c]) | ((unsigned)__builtin_bit_cast(uint16_t, gv[1][c]) << 16);
+        o.y = (unsigned)__builtin_bit_cast(uint16_t, gv[2][c]) | ((unsigned)__builtin_bit_cast(uint16_t, gv[3][c]) << 16);
+        *reinterpret_cast<uint2*>(&s_gp[0][gcol + c][4 * mg]) = o;
+      } else {
+        float x[4] = {(float)gv[0][c], (float)gv[1][c], (float)gv[2][c], (float)gv[3][c]};
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          const unsigned lo = bf16_pair(x[0], x[1]), hi = bf16_pair(x[2], x[3]);
+          *reinterpret_cast<uint2*>(&s_gp[p][gcol + c][4 * mg]) = make_uint2(lo, hi);
+          if (p + 1 < NP) {
+            x[0] -= __uint_as_float(lo << 16);
+            x[1] -= __uint_as_float(lo & 0xffff0000u);
+            x[2] -= __uint_as_float(hi << 16);
+            x[3] -= __uint_as_float(hi & 0xffff0000u);
+          }
         }
       }
     }
   };
 
-  const int wk = (wave >> 1) * 64, wn = (wave & 1) * 64;
-  v16f acc[2][2];
+  const int wk = (wave >> 1) * (S::KT / 2), wn = (wave & 1) * 64;
+  v16f acc[MI][2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < MI; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
+  const bool active = k0 + wk < a.K && n0 + wn < a.N;           // else nothing of this wave's part lies inside gW
 
-  int64_t next_ids = -1;
+  int64_t id_a = 0, id_g = 0;
   if constexpr (MAPPED) {
     if (wave == 0) {
-      s_ids[0][lane >> 5][lane & 31] = fetch_ids(0);
-      s_ids[1][lane >> 5][lane & 31] = fetch_ids(1);
-      next_ids = fetch_ids(2);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) put(t, map_a[clamped(t)], map_g[clamped(t)]);
+      id_a = map_a[clamped(2)];
+      id_g = map_g[clamped(2)];
     }
     __syncthreads();
   }
   load(0);
   for (int t = 0; t < steps; ++t) {
+    put_exp(t);
     __syncthreads();                                     // every wave is done with the step before
-    stage();
+    stage(t);
     if constexpr (MAPPED) {
-      if (wave == 0) s_ids[(t + 2) % 3][lane >> 5][lane & 31] = next_ids;
+      if (wave == 0) put(t + 2, id_a, id_g);
     }
-    __syncthreads();                                     // the step is staged, row numbers of t + 2 are there
-    if (t + 1 < steps) load(t + 1);
+    __syncthreads();                                     // the step is staged, the rows of t + 2 are known
+    load(t + 1);
     if constexpr (MAPPED) {
-      if (wave == 0) next_ids = fetch_ids(t + 3);
-    }
-#pragma unroll
-    for (int ms = 0; ms < kPwRows / 16; ++ms) {
-      const int m = ms * 16 + (lane >> 5) * 8;
-      v8bf fa[2], fg[NP][2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        fa[i] = *reinterpret_cast<const v8bf*>(&s_a[wk + 32 * i + (lane & 31)][m]);
-#pragma unroll
-        for (int p = 0; p < NP; ++p) fg[p][i] = *reinterpret_cast<const v8bf*>(&s_g[p][wn + 32 * i + (lane & 31)][m]);
+      if (wave == 0) {
+        id_a = map_a[clamped(t + 3)];
+        id_g = map_g[clamped(t + 3)];
       }
+    }
+#pragma unroll
+    for (int ms = 0; ms < ROWS / 16; ++ms) {
+      if (!active) break;
+      const int m = ms * 16 + (lane >> 5) * 8;
+      v8bf fa[MI], fg[NP][2];
+#pragma unroll
+      for (int i = 0; i < MI; ++i) fa[i] = *reinterpret_cast<const v8bf*>(&s_a[wk + 32 * i + (lane & 31)][m]);
+#pragma unroll
+      for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) fg[p][j] = *reinterpret_cast<const v8bf*>(&s_gp[p][kPwFront + wn + 32 * j + (lane & 31)][m]);
 #pragma unroll
       for (int p = NP - 1; p >= 0; --p)                  // the small parts first
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < MI; ++i)
 #pragma unroll
           for (int j = 0; j < 2; ++j)
-            if (k0 + wk + 32 * i < a.K && n0 + wn + 32 * j < a.N)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fg[p][j], acc[i][j], 0, 0, 0);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fg[p][j], acc[i][j], 0, 0, 0);
     }
   }
   float* const part = a.partial + (size_t)chunk * (size_t)a.K * (size_t)a.N;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < MI; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int col = n0 + wn + 32 * j + (lane & 31);
@@ -241,14 +338,15 @@ __global__ __launch_bounds__(kPwThreads, kPwBlocksPerCu) void packed_wgrad_kerne
     }
 }
 
-// gw[r] = sum of the partial tiles of segment r's chunks: kPwSlices runs of chunks, each added by one
-// thread per element, the runs in order.
-constexpr int kPwElems = 16, kPwSlices = 16;
-
-__global__ __launch_bounds__(kPwElems * kPwSlices) void packed_wgrad_sums_kernel(PwArgs a, float* __restrict__ gw, int64_t kn) {
-  __shared__ float s[kPwSlices][kPwElems + 1];
-  const int el = threadIdx.x % kPwElems, slice = threadIdx.x / kPwElems, r = blockIdx.y;
-  const int64_t e = (int64_t)blockIdx.x * kPwElems + el;
+// gw[r] = sum of the partial tiles of segment r's chunks: SL runs of chunks, each added by one thread per
+// V consecutive elements, the runs in order.
+template <int V, int SL>
+__global__ __launch_bounds__(256) void packed_wgrad_sums_kernel(PwArgs a, float* __restrict__ gw, int64_t kn) {
+  constexpr int EL = 256 / SL;
+  typedef float vec_t __attribute__((ext_vector_type(V)));
+  __shared__ vec_t s[SL][EL];
+  const int el = threadIdx.x % EL, slice = threadIdx.x / EL, r = blockIdx.y;
+  const int64_t e = ((int64_t)blockIdx.x * EL + el) * V;
   int64_t first = 0, b, end;
   for (int q = 0; q < r; ++q) {
     pw_segment(a.seg, a.M, q, b, end);
@@ -257,28 +355,34 @@ __global__ __launch_bounds__(kPwElems * kPwSlices) void packed_wgrad_sums_kernel
   pw_segment(a.seg, a.M, r, b, end);
   int64_t last = first + pw_chunks(b, end, a.rows_per_chunk);
   last = last < a.chunks ? last : a.chunks;
-  const int64_t per = last > first ? (last - first + kPwSlices - 1) / kPwSlices : 0;
+  const int64_t per = last > first ? (last - first + SL - 1) / SL : 0;
   const int64_t c0 = first + slice * per, c1 = c0 + per < last ? c0 + per : last;
-  float acc = 0.f;
+  vec_t acc = 0.f;
   if (e < kn) {
     const float* const p = a.partial + e;
 #pragma unroll 8
-    for (int64_t c = c0; c < c1; ++c) acc += p[(size_t)c * kn];
+    for (int64_t c = c0; c < c1; ++c) acc += *reinterpret_cast<const vec_t*>(p + (size_t)c * kn);
   }
   s[slice][el] = acc;
   __syncthreads();
   if (slice == 0 && e < kn) {
-    for (int q = 1; q < kPwSlices; ++q) acc += s[q][el];
-    gw[(size_t)r * kn + e] = acc;
+#pragma unroll
+    for (int q = 1; q < SL; ++q) acc += s[q][el];
+    *reinterpret_cast<vec_t*>(gw + (size_t)r * kn + e) = acc;
   }
 }
 
-// Rows per chunk: one round of blocks on the chip where a chunk is short (its 64 KB partial tile is
-// written and read again, which a chunk should outweigh), up to four rounds where it is long (a last
-// round that is not full then costs little).  A segment's last chunk is ragged: R of them per tile.
+typedef PwShape<128, 32, 3> PwNarrow;
+typedef PwShape<256, 32, 2> PwWide;
+
+bool pw_wide(int K) { return K > kPwTile; }
+
+// Rows per chunk: one round of blocks on the chip where a chunk is short (its partial tile is written
+// and read again, which a chunk should outweigh), up to four rounds where it is long (a last round
+// that is not full then costs little).  A segment's last chunk is ragged: R of them per tile.
 int64_t pw_chunk_rows(int64_t M, int K, int N, int R) {
-  const int64_t tiles = ceil_div(K, kPwTile) * ceil_div(N, kPwTile);
-  const int64_t slots = 256 * kPwBlocksPerCu;
+  const int64_t tiles = ceil_div(K, pw_wide(K) ? PwWide::KT : PwNarrow::KT) * ceil_div(N, kPwTile);
+  const int64_t slots = 256 * (pw_wide(K) ? PwWide::BLOCKS : PwNarrow::BLOCKS);
   auto fill = [&](int64_t rounds) {                       // rows so that about `rounds` rounds are full
     int64_t chunks = ceil_div(slots * rounds, tiles) - R;
     if (chunks < 1) chunks = 1;
@@ -287,12 +391,39 @@ int64_t pw_chunk_rows(int64_t M, int K, int N, int R) {
   const int64_t longest = fill(1), shortest = fill(4);
   int64_t rows = 2048;
   rows = rows > longest ? longest : rows < shortest ? shortest : rows;
-  rows = ceil_div(rows, kPwRows) * kPwRows;
+  rows = ceil_div(rows, (int64_t)64) * 64;
   return rows < 128 ? 128 : rows;
 }
 
 int64_t pw_chunk_count(int64_t M, int K, int N, int R) {
   return ceil_div(ceil_div(M, pw_chunk_rows(M, K, N, R)) + R, kPwXcds) * kPwXcds;
+}
+
+template <int FMT, typename TG, typename S, bool TINY> void pw_launch(const PwArgs& a, int64_t chunks, hipStream_t st) {
+  const int64_t tiles = ceil_div(a.K, S::KT) * ceil_div(a.N, kPwTile);
+  const dim3 grid((unsigned)(chunks * tiles)), block(kPwThreads);
+  static_assert(S::CG <= kPwFront, "the slack in front of a tile of G");
+  if (a.src || a.dst) hipLaunchKernelGGL((packed_wgrad_kernel<FMT, TG, true, S, TINY>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((packed_wgrad_kernel<FMT, TG, false, S, TINY>), grid, block, 0, st, a);
+}
+template <int FMT, typename TG> void pw_launch_shape(const PwArgs& a, int64_t chunks, hipStream_t st) {
+  if (pw_wide(a.K)) {
+    if (a.N < PwWide::CG) pw_launch<FMT, TG, PwWide, true>(a, chunks, st);
+    else pw_launch<FMT, TG, PwWide, false>(a, chunks, st);
+  } else {
+    if (a.N < PwNarrow::CG) pw_launch<FMT, TG, PwNarrow, true>(a, chunks, st);
+    else pw_launch<FMT, TG, PwNarrow, false>(a, chunks, st);
+  }
+}
+template <int FMT> void pw_launch_type(const PwArgs& a, int g_type, int64_t chunks, hipStream_t st) {
+  if (g_type == CXG_F32) pw_launch_shape<FMT, float>(a, chunks, st);
+  else if (g_type == CXG_BF16) pw_launch_shape<FMT, bf16_t>(a, chunks, st);
+  else pw_launch_shape<FMT, f16_t>(a, chunks, st);
+}
+
+template <int V, int SL> void pw_launch_sums(const PwArgs& a, float* gw, int64_t kn, hipStream_t st) {
+  hipLaunchKernelGGL((packed_wgrad_sums_kernel<V, SL>), dim3((unsigned)ceil_div(kn, V * (256 / SL)), (unsigned)a.R), dim3(256), 0,
+                     st, a, gw, kn);
 }
 
 }  // namespace
@@ -314,7 +445,7 @@ int cxg_packed_wgrad(const uint8_t* codes, const uint8_t* exps, int fmt, int64_t
   CXG_REQUIRE(value_type_ok(g_type), CXG_ERR_ARG, "unknown value type");
   CXG_REQUIRE(gw, CXG_ERR_ARG, "null gw");
   CXG_REQUIRE(seg_ptr || R == 1, CXG_ERR_ARG, "several segments need seg_ptr");
-  CXG_REQUIRE(M == 0 || (codes && exps && g), CXG_ERR_ARG, "null codes/exps/g");
+  CXG_REQUIRE(M == 0 || (codes && exps && g && a_rows > 0 && g_rows > 0), CXG_ERR_ARG, "null codes/exps/g, or no rows");
   CXG_REQUIRE(ldg >= 0, CXG_ERR_ARG, "negative row stride");
   CXG_REQUIRE(K <= kPrMaxCols && N <= kPrMaxCols && R <= 65535, CXG_ERR_UNSUPPORTED, "K, N or R too large");
   CXG_REQUIRE(((uintptr_t)codes & 15) == 0, CXG_ERR_ARG, "codes must be 16-byte aligned");
@@ -327,34 +458,23 @@ int cxg_packed_wgrad(const uint8_t* codes, const uint8_t* exps, int fmt, int64_t
   CXG_REQUIRE(((uintptr_t)workspace & 255) == 0, CXG_ERR_WORKSPACE, "workspace must be 256-byte aligned");
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const int64_t chunks = pw_chunk_count(M, K, N, R);
-  const int64_t tiles = ceil_div(K, kPwTile) * ceil_div(N, kPwTile);
+  const int64_t tiles = ceil_div(K, pw_wide(K) ? PwWide::KT : PwNarrow::KT) * ceil_div(N, kPwTile);
   CXG_REQUIRE(chunks * tiles < ((int64_t)1 << 31), CXG_ERR_UNSUPPORTED, "too many tiles for one launch");
   const PwArgs a{codes, exps, a_rows, g, ldg, g_rows, src_idx, dst_idx, seg_ptr, M, K, N, R, packed_pitch(K), packed_groups(K),
                  pw_chunk_rows(M, K, N, R), chunks, static_cast<float*>(workspace)};
-  const bool mapped = src_idx || dst_idx;
-#define CXG_PW_LAUNCH(FMT, TG)                                                                             \
-  do {                                                                                                     \
-    if (mapped) hipLaunchKernelGGL((packed_wgrad_kernel<FMT, TG, true>), grid, block, 0, st, a);           \
-    else hipLaunchKernelGGL((packed_wgrad_kernel<FMT, TG, false>), grid, block, 0, st, a);                 \
-  } while (0)
   if (M > 0) {
-    const dim3 grid((unsigned)(chunks * tiles)), block(kPwThreads);
-    if (fmt == CXG_PACK_INT8) {
-      if (g_type == CXG_F32) CXG_PW_LAUNCH(CXG_PACK_INT8, float);
-      else if (g_type == CXG_BF16) CXG_PW_LAUNCH(CXG_PACK_INT8, bf16_t);
-      else CXG_PW_LAUNCH(CXG_PACK_INT8, f16_t);
-    } else {
-      if (g_type == CXG_F32) CXG_PW_LAUNCH(CXG_PACK_E4M3, float);
-      else if (g_type == CXG_BF16) CXG_PW_LAUNCH(CXG_PACK_E4M3, bf16_t);
-      else CXG_PW_LAUNCH(CXG_PACK_E4M3, f16_t);
-    }
+    if (fmt == CXG_PACK_INT8) pw_launch_type<CXG_PACK_INT8>(a, g_type, chunks, st);
+    else pw_launch_type<CXG_PACK_E4M3>(a, g_type, chunks, st);
     CXG_LAUNCH_CHECK("packed_wgrad_kernel");
   }
-#undef CXG_PW_LAUNCH
   const int64_t kn = (int64_t)K * N;
-  CXG_REQUIRE(ceil_div(kn, kPwElems) < ((int64_t)1 << 31), CXG_ERR_UNSUPPORTED, "gw too large for one launch");
-  hipLaunchKernelGGL(packed_wgrad_sums_kernel, dim3((unsigned)ceil_div(kn, kPwElems), (unsigned)R),
-                     dim3(kPwElems * kPwSlices), 0, st, a, gw, kn);
+  CXG_REQUIRE(kn < ((int64_t)1 << 34), CXG_ERR_UNSUPPORTED, "gw too large for one launch");
+  // many chunks per segment: sixteen runs of them, else four; four elements at a time where gw allows
+  const bool many = chunks > 64 * (int64_t)R, vec = kn % 4 == 0 && ((uintptr_t)gw & 15) == 0;
+  if (vec && many) pw_launch_sums<4, 16>(a, gw, kn, st);
+  else if (vec) pw_launch_sums<4, 4>(a, gw, kn, st);
+  else if (many) pw_launch_sums<1, 16>(a, gw, kn, st);
+  else pw_launch_sums<1, 4>(a, gw, kn, st);
   CXG_LAUNCH_CHECK("packed_wgrad_sums_kernel");
   return CXG_OK;
 }
