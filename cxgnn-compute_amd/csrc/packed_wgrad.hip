@@ -22,7 +22,7 @@
 //
 // Row numbers that come from maps are fetched by the first wave two steps ahead into a ring in LDS
 // and checked there; a row outside its matrix counts as no row.  Exponent bytes come through LDS too,
-// one load of the second wave per step.
+// one load of the first wave per step.
 #include "packed_rows.hpp"
 
 namespace cxg {
@@ -104,7 +104,7 @@ __global__ __launch_bounds__(kPwThreads, S::BLOCKS) void packed_wgrad_kernel(PwA
   __shared__ __attribute__((aligned(16))) uint16_t s_a[S::KT][PITCH];
   __shared__ __attribute__((aligned(16))) uint16_t s_gp[NP][kPwFront + kPwTile][PITCH];   // kPwFront columns of slack in front
   __shared__ __attribute__((aligned(16))) uint8_t s_exp[2][NG][ROWS];                     // exponent bytes of a step's rows
-  __shared__ int64_t s_off[MAPPED ? 3 : 1][3][MAPPED ? ROWS : 1];                         // ring: offsets of the rows of codes, exps, g
+  __shared__ int64_t s_off[MAPPED ? 3 : 1][2][MAPPED ? ROWS : 1];                         // ring: offsets of the rows of codes and g
   __shared__ unsigned long long s_live[3];                                                // and which of them are there
   const int n_ct = (a.N + kPwTile - 1) / kPwTile, n_kt = (a.K + S::KT - 1) / S::KT, n_tile = n_ct * n_kt;
   const int64_t slot = blockIdx.x / kPwXcds;
@@ -131,11 +131,12 @@ __global__ __launch_bounds__(kPwThreads, S::BLOCKS) void packed_wgrad_kernel(PwA
   if (!TINY && ng + CG > a.N) ng = a.N - CG;                    // N >= CG
   const int gcol = TINY ? kPwFront + CG * cg : kPwFront + ng - n0 < 0 ? 0 : kPwFront + ng - n0;
   const TG* const g_base = static_cast<const TG*>(a.g) + (TINY ? 0 : ng);
-  // exponent bytes: lane of the second wave -> (group, row)
+  // exponent bytes: lane of the first wave -> (group, row)
   const int e_grp = (k0 / kPrGroup + lane / ROWS) < a.groups ? k0 / kPrGroup + lane / ROWS : a.groups - 1;
   unsigned code[4][CA / 4];
   TG gv[4][CG];
-  unsigned expo[(NG * ROWS + 63) / 64];
+  unsigned expo = 0;
+  static_assert(NG * ROWS <= 64, "one exponent byte per lane");
 
   auto load_row = [&](int i, int64_t oa, int64_t og) {
     typedef unsigned piece_t __attribute__((ext_vector_type(CA / 4)));
@@ -163,7 +164,8 @@ __global__ __launch_bounds__(kPwThreads, S::BLOCKS) void packed_wgrad_kernel(PwA
     const int64_t at = row0 + (int64_t)t * ROWS + (lane & (ROWS - 1));
     return at < row_end ? at : row_end - 1;
   };
-  auto put = [&](int t, int64_t ia, int64_t ig) {
+  // (and returns the offset of the row's exponent bytes)
+  auto put = [&](int t, int64_t ia, int64_t ig) -> int64_t {
     const int64_t at = row0 + (int64_t)t * ROWS + (lane & (ROWS - 1));
     ia = a.src ? ia : at;
     ig = a.dst ? ig : at;
@@ -171,41 +173,34 @@ __global__ __launch_bounds__(kPwThreads, S::BLOCKS) void packed_wgrad_kernel(PwA
     const unsigned long long live = __ballot(ok);
     if (lane < ROWS) {
       s_off[t % 3][0][lane] = ok ? ia * a.pitch : 0;
-      s_off[t % 3][1][lane] = ok ? ia * a.groups : 0;
-      s_off[t % 3][2][lane] = ok ? ig * a.ldg : 0;
+      s_off[t % 3][1][lane] = ok ? ig * a.ldg : 0;
     }
     if (lane == 0) s_live[t % 3] = live;
+    return ok ? ia * a.groups : 0;
   };
   // rows of step t into registers; behind the last step the last one again
-  auto load = [&](int t) {
+  auto load = [&](int t, int64_t off_exp) {
     t = t < steps ? t : steps - 1;
     const int64_t first = row0 + (int64_t)t * ROWS;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (MAPPED) {
-        load_row(i, s_off[t % 3][0][4 * mg + i], s_off[t % 3][2][4 * mg + i]);
+        load_row(i, s_off[t % 3][0][4 * mg + i], s_off[t % 3][1][4 * mg + i]);
       } else {
         const int64_t r = first + 4 * mg + i < row_end ? first + 4 * mg + i : row0;
         load_row(i, r * a.pitch, r * a.ldg);
       }
     }
-    if (wave == 1) {
-#pragma unroll
-      for (int q = 0; q < (NG * ROWS + 63) / 64; ++q) {
+    if (wave == 0) {
+      if constexpr (!MAPPED) {
         const int row = lane & (ROWS - 1);
-        int64_t o;
-        if constexpr (MAPPED) o = s_off[t % 3][1][row];
-        else o = (first + row < row_end ? first + row : row0) * a.groups;
-        expo[q] = a.exps[o + (ROWS == 64 ? (e_grp + q < a.groups ? e_grp + q : a.groups - 1) : e_grp)];
+        off_exp = (first + row < row_end ? first + row : row0) * a.groups;
       }
+      expo = a.exps[off_exp + e_grp];
     }
   };
   auto put_exp = [&](int t) {
-    if (wave == 1) {
-#pragma unroll
-      for (int q = 0; q < (NG * ROWS + 63) / 64; ++q)
-        if (q * 64 + lane < NG * ROWS) s_exp[t & 1][ROWS == 64 ? q : lane / ROWS][lane & (ROWS - 1)] = (uint8_t)expo[q];
-    }
+    if (wave == 0 && lane < NG * ROWS) s_exp[t & 1][lane / ROWS][lane & (ROWS - 1)] = (uint8_t)expo;
   };
   auto stage = [&](int t) {
     unsigned exps = *reinterpret_cast<const unsigned*>(&s_exp[t & 1][NG == 1 ? 0 : CA * cg / kPrGroup][4 * mg]);
@@ -278,26 +273,27 @@ __global__ __launch_bounds__(kPwThreads, S::BLOCKS) void packed_wgrad_kernel(PwA
       for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
   const bool active = k0 + wk < a.K && n0 + wn < a.N;           // else nothing of this wave's part lies inside gW
 
-  int64_t id_a = 0, id_g = 0;
+  int64_t id_a = 0, id_g = 0, off_now = 0, off_next = 0;
   if constexpr (MAPPED) {
     if (wave == 0) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) put(t, map_a[clamped(t)], map_g[clamped(t)]);
+      off_now = put(0, map_a[clamped(0)], map_g[clamped(0)]);
+      off_next = put(1, map_a[clamped(1)], map_g[clamped(1)]);
       id_a = map_a[clamped(2)];
       id_g = map_g[clamped(2)];
     }
     __syncthreads();
   }
-  load(0);
+  load(0, off_now);
   for (int t = 0; t < steps; ++t) {
     put_exp(t);
     __syncthreads();                                     // every wave is done with the step before
     stage(t);
     if constexpr (MAPPED) {
-      if (wave == 0) put(t + 2, id_a, id_g);
+      off_now = off_next;
+      if (wave == 0) off_next = put(t + 2, id_a, id_g);
     }
     __syncthreads();                                     // the step is staged, the rows of t + 2 are known
-    load(t + 1);
+    load(t + 1, off_now);
     if constexpr (MAPPED) {
       if (wave == 0) {
         id_a = map_a[clamped(t + 3)];
@@ -372,7 +368,11 @@ __global__ __launch_bounds__(256) void packed_wgrad_sums_kernel(PwArgs a, float*
   }
 }
 
-typedef PwShape<128, 32, 3> PwNarrow;
+// Inputs of at most 128 columns: 128 x 128 tiles, 64 rows per step, two blocks per CU (32 rows and three
+// blocks: 114 against 97 us for 1 M rows x 128 x 128 of 16 types in bf16, 55 against 50 us for 169,343 x
+// 128 x 256 in fp32).  Wider inputs: 256 x 128 tiles, so that a step of G is staged once per 256 columns
+// of A (2.33 M x 512 x 512 in fp32).
+typedef PwShape<128, 64, 2> PwNarrow;
 typedef PwShape<256, 32, 2> PwWide;
 
 bool pw_wide(int K) { return K > kPwTile; }
@@ -380,8 +380,10 @@ bool pw_wide(int K) { return K > kPwTile; }
 // Rows per chunk: one round of blocks on the chip where a chunk is short (its partial tile is written
 // and read again, which a chunk should outweigh), up to four rounds where it is long (a last round
 // that is not full then costs little).  A segment's last chunk is ragged: R of them per tile.
+int64_t pw_tiles(int K, int N) { return ceil_div(K, pw_wide(K) ? PwWide::KT : kPwTile) * ceil_div(N, kPwTile); }
+
 int64_t pw_chunk_rows(int64_t M, int K, int N, int R) {
-  const int64_t tiles = ceil_div(K, pw_wide(K) ? PwWide::KT : PwNarrow::KT) * ceil_div(N, kPwTile);
+  const int64_t tiles = pw_tiles(K, N);
   const int64_t slots = 256 * (pw_wide(K) ? PwWide::BLOCKS : PwNarrow::BLOCKS);
   auto fill = [&](int64_t rounds) {                       // rows so that about `rounds` rounds are full
     int64_t chunks = ceil_div(slots * rounds, tiles) - R;
@@ -458,7 +460,7 @@ int cxg_packed_wgrad(const uint8_t* codes, const uint8_t* exps, int fmt, int64_t
   CXG_REQUIRE(((uintptr_t)workspace & 255) == 0, CXG_ERR_WORKSPACE, "workspace must be 256-byte aligned");
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const int64_t chunks = pw_chunk_count(M, K, N, R);
-  const int64_t tiles = ceil_div(K, pw_wide(K) ? PwWide::KT : PwNarrow::KT) * ceil_div(N, kPwTile);
+  const int64_t tiles = pw_tiles(K, N);
   CXG_REQUIRE(chunks * tiles < ((int64_t)1 << 31), CXG_ERR_UNSUPPORTED, "too many tiles for one launch");
   const PwArgs a{codes, exps, a_rows, g, ldg, g_rows, src_idx, dst_idx, seg_ptr, M, K, N, R, packed_pitch(K), packed_groups(K),
                  pw_chunk_rows(M, K, N, R), chunks, static_cast<float*>(workspace)};
