@@ -300,6 +300,7 @@ __global__ __launch_bounds__(kPwThreads, S::BLOCKS) void packed_wgrad_kernel(PwA
         id_g = map_g[clamped(t + 3)];
       }
     }
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int ms = 0; ms < ROWS / 16; ++ms) {
       if (!active) break;
@@ -319,6 +320,7 @@ __global__ __launch_bounds__(kPwThreads, S::BLOCKS) void packed_wgrad_kernel(PwA
           for (int j = 0; j < 2; ++j)
             acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fg[p][j], acc[i][j], 0, 0, 0);
     }
+    __builtin_amdgcn_s_setprio(0);
   }
   float* const part = a.partial + (size_t)chunk * (size_t)a.K * (size_t)a.N;
 #pragma unroll
@@ -378,7 +380,7 @@ typedef PwShape<256, 32, 2> PwWide;
 bool pw_wide(int K) { return K > kPwTile; }
 
 // Rows per chunk: one round of blocks on the chip where a chunk is short (its partial tile is written
-// and read again, which a chunk should outweigh), up to four rounds where it is long (a last round
+// and read again, which a chunk should outweigh), up to two rounds where it is long (a last round
 // that is not full then costs little).  A segment's last chunk is ragged: R of them per tile.
 int64_t pw_tiles(int K, int N) { return ceil_div(K, pw_wide(K) ? PwWide::KT : kPwTile) * ceil_div(N, kPwTile); }
 
@@ -390,7 +392,7 @@ int64_t pw_chunk_rows(int64_t M, int K, int N, int R) {
     if (chunks < 1) chunks = 1;
     return ceil_div(M, chunks);
   };
-  const int64_t longest = fill(1), shortest = fill(4);
+  const int64_t longest = fill(1), shortest = fill(2);
   int64_t rows = 2048;
   rows = rows > longest ? longest : rows < shortest ? shortest : rows;
   rows = ceil_div(rows, (int64_t)64) * 64;

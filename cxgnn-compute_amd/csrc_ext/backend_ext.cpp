@@ -1237,6 +1237,53 @@ Tensor packed_wgrad(const Tensor& codes, const Tensor& exps, int64_t cols, int64
   return gw;
 }
 
+// x W^T + bias (+ addend) with the library's product, its input kept for the weight gradient in 8 bits:
+// the compiled node of PackedLinearOP (cxgnncomp/graph_conv.py) for the shapes that the split GEMM does
+// not take, where the host's time is what counts.
+Tensor column_sum(const Tensor& g) {
+  if (g.scalar_type() != at::kFloat) return g.sum(0);
+  const Tensor x = g.contiguous();
+  Tensor out = torch::empty({x.size(1)}, x.options().requires_grad(false));
+  Tensor ws = workspace(cxg_batchnorm_workspace_bytes(x.size(0), (int)x.size(1)), x);
+  c10::DeviceGuard guard(x.device());
+  check(cxg_column_sum_f32((const float*)ptr_or_null(x), x.size(0), (int)x.size(1), x.stride(0), (float*)out.data_ptr(), ws.data_ptr(),
+                           (size_t)ws.numel(), stream_of(x)));
+  return out;
+}
+
+struct PackedLinearFunction : public torch::autograd::Function<PackedLinearFunction> {
+  static Tensor forward(AutogradContext* ctx, Tensor x, Tensor weight, OptTensor bias, OptTensor addend, int64_t fmt) {
+    const std::vector<int64_t> need = {x.requires_grad(), weight.requires_grad(), bias.has_value() && bias->requires_grad(),
+                                       addend.has_value() && addend->requires_grad()};
+    tensor_list saved = {weight, Tensor(), Tensor()};
+    if (need[1]) std::tie(saved[1], saved[2]) = pack_rows(x.reshape({-1, x.size(-1)}), fmt);
+    ctx->save_for_backward(saved);
+    ctx->saved_data["how"] = std::vector<int64_t>{fmt, x.size(-1), need[0], need[1], need[2], need[3]};
+    if (!addend.has_value()) return at::linear(x, weight, bias);
+    Tensor out = at::addmm(*addend, x, weight.t());
+    return bias.has_value() ? out.add_(*bias) : out;
+  }
+
+  static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+    if (at::GradMode::is_enabled()) throw std::runtime_error("linear(checkpoint=) has no second derivatives (create_graph=True)");
+    const auto saved = ctx->get_saved_variables();
+    const std::vector<int64_t> how = ctx->saved_data["how"].toIntVector();
+    const Tensor &weight = saved[0], g = grads[0];
+    const Tensor rows = g.reshape({-1, g.size(-1)});
+    tensor_list out(5);
+    if (how[2]) out[0] = at::matmul(g, weight);
+    if (how[3])
+      out[1] = packed_wgrad(saved[1], saved[2], how[1], how[0], rows, c10::nullopt, c10::nullopt, c10::nullopt)[0].t().to(weight.scalar_type());
+    if (how[4]) out[2] = column_sum(rows);
+    if (how[5]) out[3] = g;
+    return out;
+  }
+};
+
+Tensor packed_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& addend, int64_t fmt) {
+  return PackedLinearFunction::apply(x, weight, bias, addend, fmt);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1260,6 +1307,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("head_sum", &head_sum);
   m.def("pack_rows", &pack_rows, py::arg("x"), py::arg("fmt"));
   m.def("unpack_rows", &unpack_rows, py::arg("codes"), py::arg("exps"), py::arg("cols"), py::arg("fmt"), py::arg("dtype"));
+  m.def("packed_linear", &packed_linear, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("addend"), py::arg("fmt"));
   m.def("packed_wgrad", &packed_wgrad, py::arg("codes"), py::arg("exps"), py::arg("cols"), py::arg("fmt"), py::arg("g"),
         py::arg("seg_ptr") = py::none(), py::arg("src_idx") = py::none(), py::arg("dst_idx") = py::none());
   m.def("residual_norm", &residual_norm, py::arg("x"), py::arg("f"), py::arg("gate"), py::arg("post"), py::arg("post_weight"),

@@ -20,7 +20,7 @@ from cxgnncomp_backend import (aggr_rel, aggr_rgcn_direct_func, edge_attention, 
                                selective_aggr, selective_aggr_bwd)
 
 from .graph_kernel import SpMMValOP
-from .packed import PackedRows, check_format, pack_rows, packed_weight_grad
+from .packed import FORMATS, PackedRows, check_format, pack_rows, packed_weight_grad
 from .timer import TimerOP
 from .typed_linear import (TypedLinearE2EOP, TypedLinearS2DAggrMMOP, TypedLinearS2DMMAggrOP,
                            TypedLinearS2DPushOP, TypedLinearS2DSort)
@@ -512,6 +512,10 @@ def linear(x, weight, bias=None, addend=None, checkpoint=None):
     if check_format(checkpoint) is not None and x.is_cuda:
         if addend is not None and x.dim() != 2:
             raise ValueError("an addend goes with x [N, C]")
+        rows, (n, k) = x.numel() // max(1, x.shape[-1]), weight.shape
+        if not (_typed.dense_linear_shape(rows, k, n, bias is None and addend is None)
+                or _typed.dense_linear_shape(rows, n, k, True)):
+            return _ops._C.packed_linear(x, weight, bias, addend, FORMATS[checkpoint])     # library products: the compiled node
         return PackedLinearOP.apply(x, weight, bias, addend, checkpoint)
     if not x.is_cuda or (addend is not None and x.dim() != 2):
         out = F.linear(x, weight, bias)

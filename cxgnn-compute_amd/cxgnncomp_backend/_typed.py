@@ -162,6 +162,18 @@ def _one_segment(m_rows, device):
     return seg
 
 
+def dense_linear_shape(M, K, N, plain):
+    """Whether ``dense_linear`` takes x [M, K] @ w [K, N]; ``plain``: without bias and addend."""
+    # the 256-wide form stores from the accumulators (no staged 16-byte stores): it beats the
+    # library from about 10^5 rows on (measured on 4 k - 2.4 M rows, with and without addend)
+    wide = 176 <= K <= 256 and N >= 96 and M >= DENSE_WIDE_MIN_ROWS
+    # the tiled kernel has no epilogue; without one it also takes K above 256 (2.33 M x 512 x 512: 4.0 ms
+    # against 8.6 ms in the library)
+    tiled = plain and K > 256 and M >= DENSE_WIDE_MIN_ROWS
+    return (_PRECISION_FLAGS.get(GEMM_PRECISION, 0) == GEMM_SPLIT_F16X3 and M >= DENSE_MIN_ROWS and K % 4 == 0
+            and (K <= 128 or wide or tiled))
+
+
 def dense_linear(x, w_kn, bias=None, addend=None):
     """x [M, K] @ w_kn [K, N] + bias [N] + addend [M, N] (either may be None) as a typed GEMM over
     one segment, bias and addend added to the accumulator before the rows are stored.  Returns
@@ -170,17 +182,11 @@ def dense_linear(x, w_kn, bias=None, addend=None):
     10^5 rows; any K without bias and addend from 10^5 rows on: the tiled kernel), K not a multiple
     of 4, a default precision other than the fp16 split form."""
     flags = _PRECISION_FLAGS.get(GEMM_PRECISION, 0)
-    if flags != GEMM_SPLIT_F16X3 or not x.is_cuda or x.dim() != 2 or x.dtype != torch.float32 or w_kn.dtype != torch.float32:
+    if not x.is_cuda or x.dim() != 2 or x.dtype != torch.float32 or w_kn.dtype != torch.float32:
         return None
     M, K = x.shape
     N = w_kn.shape[1]
-    # the 256-wide form stores from the accumulators (no staged 16-byte stores): it beats the
-    # library from about 10^5 rows on (measured on 4 k - 2.4 M rows, with and without addend)
-    wide = 176 <= K <= 256 and N >= 96 and M >= DENSE_WIDE_MIN_ROWS
-    # the tiled kernel has no epilogue; without one it also takes K above 256 (2.33 M x 512 x 512: 4.0 ms
-    # against 8.6 ms in the library)
-    tiled = (bias is None and addend is None and K > 256 and K % 4 == 0 and M >= DENSE_WIDE_MIN_ROWS)
-    if M < DENSE_MIN_ROWS or K % 4 or not (K <= 128 or wide or tiled) or w_kn.shape[0] != K:
+    if not dense_linear_shape(M, K, N, bias is None and addend is None) or w_kn.shape[0] != K:
         return None
     if not x.is_contiguous() or x.data_ptr() % 16:
         return None
