@@ -56,7 +56,8 @@ struct PwArgs {
   int64_t M;
   int K, N, R, pitch, groups;
   int64_t rows_per_chunk, chunks;
-  float* partial;
+  float* partial;          // [chunks][K * N], then N column sums of G if they are wanted
+  int64_t stride;          // floats per chunk
 };
 
 template <typename TG> struct PwParts;
@@ -202,6 +203,10 @@ __global__ __launch_bounds__(kPwThreads, S::BLOCKS) void packed_wgrad_kernel(PwA
   auto put_exp = [&](int t) {
     if (wave == 0 && lane < NG * ROWS) s_exp[t & 1][lane / ROWS][lane & (ROWS - 1)] = (uint8_t)expo;
   };
+  const bool sums = a.stride > (int64_t)a.K * a.N && k0 == 0;    // this block also adds up the rows of its columns of G
+  float colsum[CG];
+#pragma unroll
+  for (int c = 0; c < CG; ++c) colsum[c] = 0.f;
   auto stage = [&](int t) {
     unsigned exps = *reinterpret_cast<const unsigned*>(&s_exp[t & 1][NG == 1 ? 0 : CA * cg / kPrGroup][4 * mg]);
     unsigned live;                                       // which of this thread's four rows are there
@@ -237,6 +242,10 @@ __global__ __launch_bounds__(kPwThreads, S::BLOCKS) void packed_wgrad_kernel(PwA
       for (int c = 0; c < 4; ++c)
         *reinterpret_cast<uint2*>(&s_a[CA * cg + 4 * q + c][4 * mg]) =
             make_uint2(bf16_pair(v[0][c], v[1][c]), bf16_pair(v[2][c], v[3][c]));
+    }
+    if (sums) {
+#pragma unroll
+      for (int c = 0; c < CG; ++c) colsum[c] += ((float)gv[0][c] + (float)gv[1][c]) + ((float)gv[2][c] + (float)gv[3][c]);
     }
 #pragma unroll
     for (int c = 0; c < CG; ++c) {
@@ -322,7 +331,22 @@ __global__ __launch_bounds__(kPwThreads, S::BLOCKS) void packed_wgrad_kernel(PwA
     }
     __builtin_amdgcn_s_setprio(0);
   }
-  float* const part = a.partial + (size_t)chunk * (size_t)a.K * (size_t)a.N;
+  float* const part = a.partial + (size_t)chunk * (size_t)a.stride;
+  if (sums) {
+    // over the groups of four rows, through the LDS that held G (a column that two threads hold, they hold alike)
+    float (*const s_sum)[kPwFront + kPwTile] = reinterpret_cast<float (*)[kPwFront + kPwTile]>(&s_gp[0][0][0]);
+    static_assert(sizeof(float) * MG * (kPwFront + kPwTile) <= sizeof(s_gp), "the sums fit");
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < CG; ++c) s_sum[mg][gcol + c] = colsum[c];
+    __syncthreads();
+    if (tid < kPwTile && n0 + tid < a.N) {
+      float v = 0.f;
+#pragma unroll
+      for (int q = 0; q < MG; ++q) v += s_sum[q][kPwFront + tid];
+      part[(size_t)a.K * a.N + n0 + tid] = v;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -336,10 +360,10 @@ __global__ __launch_bounds__(kPwThreads, S::BLOCKS) void packed_wgrad_kernel(PwA
     }
 }
 
-// gw[r] = sum of the partial tiles of segment r's chunks: SL runs of chunks, each added by one thread per
-// V consecutive elements, the runs in order.
+// gw[r] (and the column sums gb[r]) = sum of the partial results of segment r's chunks: SL runs of chunks,
+// each added by one thread per V consecutive elements, the runs in order.
 template <int V, int SL>
-__global__ __launch_bounds__(256) void packed_wgrad_sums_kernel(PwArgs a, float* __restrict__ gw, int64_t kn) {
+__global__ __launch_bounds__(256) void packed_wgrad_sums_kernel(PwArgs a, float* __restrict__ gw, float* __restrict__ gb) {
   constexpr int EL = 256 / SL;
   typedef float vec_t __attribute__((ext_vector_type(V)));
   __shared__ vec_t s[SL][EL];
@@ -356,17 +380,19 @@ __global__ __launch_bounds__(256) void packed_wgrad_sums_kernel(PwArgs a, float*
   const int64_t per = last > first ? (last - first + SL - 1) / SL : 0;
   const int64_t c0 = first + slice * per, c1 = c0 + per < last ? c0 + per : last;
   vec_t acc = 0.f;
-  if (e < kn) {
+  if (e < a.stride) {
     const float* const p = a.partial + e;
 #pragma unroll 8
-    for (int64_t c = c0; c < c1; ++c) acc += *reinterpret_cast<const vec_t*>(p + (size_t)c * kn);
+    for (int64_t c = c0; c < c1; ++c) acc += *reinterpret_cast<const vec_t*>(p + (size_t)c * a.stride);
   }
   s[slice][el] = acc;
   __syncthreads();
-  if (slice == 0 && e < kn) {
+  if (slice == 0 && e < a.stride) {
 #pragma unroll
     for (int q = 1; q < SL; ++q) acc += s[q][el];
-    *reinterpret_cast<vec_t*>(gw + (size_t)r * kn + e) = acc;
+    const int64_t kn = (int64_t)a.K * a.N;
+    float* const dst = e < kn ? gw + (size_t)r * kn + e : gb + (size_t)r * a.N + (e - kn);
+    *reinterpret_cast<vec_t*>(dst) = acc;
   }
 }
 
@@ -425,9 +451,9 @@ template <int FMT> void pw_launch_type(const PwArgs& a, int g_type, int64_t chun
   else pw_launch_shape<FMT, f16_t>(a, chunks, st);
 }
 
-template <int V, int SL> void pw_launch_sums(const PwArgs& a, float* gw, int64_t kn, hipStream_t st) {
-  hipLaunchKernelGGL((packed_wgrad_sums_kernel<V, SL>), dim3((unsigned)ceil_div(kn, V * (256 / SL)), (unsigned)a.R), dim3(256), 0,
-                     st, a, gw, kn);
+template <int V, int SL> void pw_launch_sums(const PwArgs& a, float* gw, float* gb, hipStream_t st) {
+  hipLaunchKernelGGL((packed_wgrad_sums_kernel<V, SL>), dim3((unsigned)ceil_div(a.stride, V * (256 / SL)), (unsigned)a.R),
+                     dim3(256), 0, st, a, gw, gb);
 }
 
 }  // namespace
@@ -437,12 +463,12 @@ extern "C" {
 
 size_t cxg_packed_wgrad_workspace_bytes(int64_t M, int K, int N, int R) {
   if (M < 0 || K < 1 || N < 1 || R < 1) return 0;
-  return (size_t)cxg::pw_chunk_count(M, K, N, R) * (size_t)K * (size_t)N * sizeof(float) + 256;
+  return (size_t)cxg::pw_chunk_count(M, K, N, R) * ((size_t)K + 1) * (size_t)N * sizeof(float) + 256;
 }
 
 int cxg_packed_wgrad(const uint8_t* codes, const uint8_t* exps, int fmt, int64_t a_rows, const void* g, int64_t ldg,
                      int g_type, int64_t g_rows, const int64_t* src_idx, const int64_t* dst_idx, const int64_t* seg_ptr,
-                     int64_t M, int K, int N, int R, float* gw, void* workspace, size_t workspace_bytes, void* stream) {
+                     int64_t M, int K, int N, int R, float* gw, float* gb, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace cxg;
   CXG_REQUIRE(M >= 0 && K >= 1 && N >= 1 && R >= 1 && a_rows >= 0 && g_rows >= 0, CXG_ERR_ARG, "bad M/K/N/R/rows");
   CXG_REQUIRE(fmt == CXG_PACK_INT8 || fmt == CXG_PACK_E4M3, CXG_ERR_ARG, "unknown 8-bit format");
@@ -465,20 +491,20 @@ int cxg_packed_wgrad(const uint8_t* codes, const uint8_t* exps, int fmt, int64_t
   const int64_t tiles = pw_tiles(K, N);
   CXG_REQUIRE(chunks * tiles < ((int64_t)1 << 31), CXG_ERR_UNSUPPORTED, "too many tiles for one launch");
   const PwArgs a{codes, exps, a_rows, g, ldg, g_rows, src_idx, dst_idx, seg_ptr, M, K, N, R, packed_pitch(K), packed_groups(K),
-                 pw_chunk_rows(M, K, N, R), chunks, static_cast<float*>(workspace)};
+                 pw_chunk_rows(M, K, N, R), chunks, static_cast<float*>(workspace), (int64_t)K * N + (gb ? N : 0)};
   if (M > 0) {
     if (fmt == CXG_PACK_INT8) pw_launch_type<CXG_PACK_INT8>(a, g_type, chunks, st);
     else pw_launch_type<CXG_PACK_E4M3>(a, g_type, chunks, st);
     CXG_LAUNCH_CHECK("packed_wgrad_kernel");
   }
-  const int64_t kn = (int64_t)K * N;
-  CXG_REQUIRE(kn < ((int64_t)1 << 34), CXG_ERR_UNSUPPORTED, "gw too large for one launch");
-  // many chunks per segment: sixteen runs of them, else four; four elements at a time where gw allows
-  const bool many = chunks > 64 * (int64_t)R, vec = kn % 4 == 0 && ((uintptr_t)gw & 15) == 0;
-  if (vec && many) pw_launch_sums<4, 16>(a, gw, kn, st);
-  else if (vec) pw_launch_sums<4, 4>(a, gw, kn, st);
-  else if (many) pw_launch_sums<1, 16>(a, gw, kn, st);
-  else pw_launch_sums<1, 4>(a, gw, kn, st);
+  CXG_REQUIRE(a.stride < ((int64_t)1 << 34), CXG_ERR_UNSUPPORTED, "gw too large for one launch");
+  // many chunks per segment: sixteen runs of them, else four; four elements at a time where the shapes allow
+  const bool many = chunks > 64 * (int64_t)R;
+  const bool vec = (int64_t)K * N % 4 == 0 && (!gb || N % 4 == 0) && (((uintptr_t)gw | (uintptr_t)gb) & 15) == 0;
+  if (vec && many) pw_launch_sums<4, 16>(a, gw, gb, st);
+  else if (vec) pw_launch_sums<4, 4>(a, gw, gb, st);
+  else if (many) pw_launch_sums<1, 16>(a, gw, gb, st);
+  else pw_launch_sums<1, 4>(a, gw, gb, st);
   CXG_LAUNCH_CHECK("packed_wgrad_sums_kernel");
   return CXG_OK;
 }

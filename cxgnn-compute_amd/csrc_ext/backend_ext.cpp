@@ -1199,9 +1199,9 @@ Tensor unpack_rows(const Tensor& codes, const Tensor& exps, int64_t cols, int64_
   return out;
 }
 
-// [R, K, N]; seg missing: one segment of all rows
-Tensor packed_wgrad(const Tensor& codes, const Tensor& exps, int64_t cols, int64_t fmt_id, const Tensor& g_in, const OptTensor& seg,
-                    const OptTensor& src, const OptTensor& dst) {
+// [R, K, N] and, with want_sums, [R, N]; seg missing: one segment of all rows
+std::tuple<Tensor, OptTensor> packed_wgrad(const Tensor& codes, const Tensor& exps, int64_t cols, int64_t fmt_id, const Tensor& g_in,
+                                           const OptTensor& seg, const OptTensor& src, const OptTensor& dst, bool want_sums) {
   req_packed(codes, exps, cols);
   const Tensor g = rows_of(g_in, "g");
   same_device(g, codes, "g");
@@ -1227,30 +1227,21 @@ Tensor packed_wgrad(const Tensor& codes, const Tensor& exps, int64_t cols, int64
     if (segs < 1) bad("seg_ptr needs at least two entries");
   }
   Tensor gw = torch::empty({segs, cols, g.size(1)}, codes.options().dtype(at::kFloat));
+  OptTensor gb;
+  if (want_sums) gb = torch::empty({segs, g.size(1)}, gw.options());
   const int K = (int)cols, N = (int)g.size(1), R = (int)segs;
   Tensor ws = workspace(cxg_packed_wgrad_workspace_bytes(rows, K, N, R), codes);
   c10::DeviceGuard guard(codes.device());
   check(cxg_packed_wgrad((const uint8_t*)ptr_or_null(codes), (const uint8_t*)ptr_or_null(exps), (int)fmt_id, codes.size(0),
                          ptr_or_null(g), g.stride(0), value_type(g, "g"), g.size(0), (const int64_t*)map_ptr(src),
                          (const int64_t*)map_ptr(dst), (const int64_t*)map_ptr(seg), rows, K, N, R, (float*)gw.data_ptr(),
-                         ws.data_ptr(), (size_t)ws.numel(), stream_of(codes)));
-  return gw;
+                         gb.has_value() ? (float*)gb->data_ptr() : nullptr, ws.data_ptr(), (size_t)ws.numel(), stream_of(codes)));
+  return std::make_tuple(gw, gb);
 }
 
 // x W^T + bias (+ addend) with the library's product, its input kept for the weight gradient in 8 bits:
 // the compiled node of PackedLinearOP (cxgnncomp/graph_conv.py) for the shapes that the split GEMM does
 // not take, where the host's time is what counts.
-Tensor column_sum(const Tensor& g) {
-  if (g.scalar_type() != at::kFloat) return g.sum(0);
-  const Tensor x = g.contiguous();
-  Tensor out = torch::empty({x.size(1)}, x.options().requires_grad(false));
-  Tensor ws = workspace(cxg_batchnorm_workspace_bytes(x.size(0), (int)x.size(1)), x);
-  c10::DeviceGuard guard(x.device());
-  check(cxg_column_sum_f32((const float*)ptr_or_null(x), x.size(0), (int)x.size(1), x.stride(0), (float*)out.data_ptr(), ws.data_ptr(),
-                           (size_t)ws.numel(), stream_of(x)));
-  return out;
-}
-
 struct PackedLinearFunction : public torch::autograd::Function<PackedLinearFunction> {
   static Tensor forward(AutogradContext* ctx, Tensor x, Tensor weight, OptTensor bias, OptTensor addend, int64_t fmt) {
     const std::vector<int64_t> need = {x.requires_grad(), weight.requires_grad(), bias.has_value() && bias->requires_grad(),
@@ -1272,9 +1263,13 @@ struct PackedLinearFunction : public torch::autograd::Function<PackedLinearFunct
     const Tensor rows = g.reshape({-1, g.size(-1)});
     tensor_list out(5);
     if (how[2]) out[0] = at::matmul(g, weight);
-    if (how[3])
-      out[1] = packed_wgrad(saved[1], saved[2], how[1], how[0], rows, c10::nullopt, c10::nullopt, c10::nullopt)[0].t().to(weight.scalar_type());
-    if (how[4]) out[2] = column_sum(rows);
+    if (how[3]) {                              // the bias gradient comes out of the same pass over g
+      auto [gw, gb] = packed_wgrad(saved[1], saved[2], how[1], how[0], rows, c10::nullopt, c10::nullopt, c10::nullopt, how[4]);
+      out[1] = gw[0].t().to(weight.scalar_type());
+      if (how[4]) out[2] = (*gb)[0].to(g.scalar_type());
+    } else if (how[4]) {
+      out[2] = rows.sum(0);
+    }
     if (how[5]) out[3] = g;
     return out;
   }
@@ -1309,7 +1304,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("unpack_rows", &unpack_rows, py::arg("codes"), py::arg("exps"), py::arg("cols"), py::arg("fmt"), py::arg("dtype"));
   m.def("packed_linear", &packed_linear, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("addend"), py::arg("fmt"));
   m.def("packed_wgrad", &packed_wgrad, py::arg("codes"), py::arg("exps"), py::arg("cols"), py::arg("fmt"), py::arg("g"),
-        py::arg("seg_ptr") = py::none(), py::arg("src_idx") = py::none(), py::arg("dst_idx") = py::none());
+        py::arg("seg_ptr") = py::none(), py::arg("src_idx") = py::none(), py::arg("dst_idx") = py::none(),
+        py::arg("want_sums") = false);
   m.def("residual_norm", &residual_norm, py::arg("x"), py::arg("f"), py::arg("gate"), py::arg("post"), py::arg("post_weight"),
         py::arg("post_bias"), py::arg("pre"), py::arg("pre_weight"), py::arg("pre_bias"), py::arg("res_scale"),
         py::arg("branch_scale"), py::arg("eps"));

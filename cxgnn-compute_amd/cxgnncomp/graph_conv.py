@@ -462,9 +462,9 @@ class LinearOP(torch.autograd.Function):
 
 class PackedLinearOP(torch.autograd.Function):
     """``LinearOP`` whose input is kept for the backward pass in 8 bits (``pack_rows``) instead of as it
-    is: a quarter of the memory of fp32 rows, half of bf16.  Output, input gradient and bias gradient
-    are LinearOP's; the weight gradient is that of the rows the 8 bits stand for, multiplied from them
-    directly (``packed_weight_grad``)."""
+    is: a quarter of the memory of fp32 rows, half of bf16.  Output and input gradient are LinearOP's;
+    the weight gradient is that of the rows the 8 bits stand for, multiplied from them directly, and
+    the bias gradient comes out of the same pass over g (``packed_weight_grad``)."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, addend, fmt):
@@ -484,9 +484,10 @@ class PackedLinearOP(torch.autograd.Function):
                 gx = g @ weight
         if ctx.needs_input_grad[1]:
             packed = PackedRows(codes, exps, ctx.shape[-1], ctx.fmt)
-            gw = packed_weight_grad(packed, g.reshape(-1, g.shape[-1]))[0].t().to(weight.dtype)
-        if ctx.needs_input_grad[2]:
-            gb = _bias_grad(g)
+            gw, gb = packed_weight_grad(packed, g.reshape(-1, g.shape[-1]), want_sums=True)
+            gw, gb = gw[0].t().to(weight.dtype), gb[0].to(g.dtype) if ctx.needs_input_grad[2] else None
+        elif ctx.needs_input_grad[2]:
+            gb = g.reshape(-1, g.shape[-1]).sum(dim=0)
         return gx, gw, gb, g if ctx.needs_input_grad[3] else None, None
 
 
@@ -498,11 +499,6 @@ def _linear_product(x, weight, bias, addend):
         return F.linear(x, weight, bias)
     out = torch.addmm(addend, x, weight.t())
     return out if bias is None else out.add_(bias)
-
-
-def _bias_grad(g):
-    g = g.reshape(-1, g.shape[-1])
-    return _ops.column_sum(g.contiguous()) if g.dtype == torch.float32 else g.sum(dim=0)
 
 
 def linear(x, weight, bias=None, addend=None, checkpoint=None):

@@ -64,12 +64,15 @@ def pack_rows(x, fmt="int8"):
     return PackedRows(codes, exps, x.shape[1], fmt, x.dtype)
 
 
-def packed_weight_grad(packed, g, seg_ptr=None, src_idx=None, dst_idx=None):
+def packed_weight_grad(packed, g, seg_ptr=None, src_idx=None, dst_idx=None, want_sums=False):
     """gW[r] = sum over the rows i of segment r of A[src_idx[i]]^T g[dst_idx[i]] -> fp32 [R, C, N], A the rows
     ``packed`` stands for, g [*, N] float32 / bfloat16 / float16.
 
     ``seg_ptr`` [R + 1] (int64, non-decreasing): rows seg_ptr[r] .. seg_ptr[r + 1] - 1 are segment r's; None: one
     segment of all rows.  The row maps (int64) may be missing: row i.  An entry outside its matrix
-    (padding) leaves the row out.  Products are exact up to fp32 accumulation, in a fixed order: results
+    (padding) leaves the row out.  ``want_sums``: returns (gW, gB), gB [R, N] the sums of the same rows of g (the
+    bias gradient), from the same pass.  Products are exact up to fp32 accumulation, in a fixed order: results
     repeat bit for bit."""
-    return _ops._C.packed_wgrad(packed.codes, packed.exps, packed.cols, FORMATS[packed.fmt], g, seg_ptr, src_idx, dst_idx)
+    gw, gb = _ops._C.packed_wgrad(packed.codes, packed.exps, packed.cols, FORMATS[packed.fmt], g, seg_ptr, src_idx, dst_idx,
+                                  want_sums)
+    return (gw, gb) if want_sums else gw

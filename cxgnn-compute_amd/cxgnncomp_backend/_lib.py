@@ -109,8 +109,8 @@ SIGNATURES = {
     "cxg_pack_rows": (_I32, [_P, _I64, _I32, _I32, _I64, _I32, _P, _P, _P]),
     "cxg_unpack_rows": (_I32, [_P, _P, _I32, _I64, _I32, _P, _I32, _P]),
     "cxg_packed_wgrad_workspace_bytes": (_SZ, [_I64, _I32, _I32, _I32]),
-    "cxg_packed_wgrad": (_I32, [_P, _P, _I32, _I64, _P, _I64, _I32, _I64, _P, _P, _P, _I64, _I32, _I32, _I32, _P, _P, _SZ,
-                                _P]),
+    "cxg_packed_wgrad": (_I32, [_P, _P, _I32, _I64, _P, _I64, _I32, _I64, _P, _P, _P, _I64, _I32, _I32, _I32, _P, _P, _P,
+                                _SZ, _P]),
 }
 
 _lib = None

@@ -816,7 +816,9 @@ int cxg_unpack_rows(const uint8_t* codes, const uint8_t* exps, int fmt, int64_t 
  * (aligned to its values).  src(i) = src_idx ? src_idx[i] : i, dst likewise; seg_ptr [R + 1] as in
  * cxg_typed_gemm_f32, NULL for one segment of all M rows (R = 1).  A row whose src or dst lies outside
  * its matrix is left out.  code * scale is a bf16 number and multiplies as it is; G goes in as one
- * (bf16), two (fp16) or three (fp32) bf16 parts that add up to it exactly, accumulation is fp32.
+ * (bf16), two (fp16) or three (fp32) bf16 parts that add up to it exactly, accumulation is fp32 (an
+ * infinity in G, or a magnitude that rounds to one in bf16, comes out as NaN or infinity).  gb (or NULL)
+ * [R, N]: sums of the same rows of G, the bias gradient, from the same pass.
  * Partial sums over row chunks are added in a fixed order: results repeat bit for bit.  The workspace
  * is 256-byte aligned.
  */
@@ -824,7 +826,7 @@ size_t cxg_packed_wgrad_workspace_bytes(int64_t M, int K, int N, int R);
 int cxg_packed_wgrad(const uint8_t* codes, const uint8_t* exps, int fmt, int64_t a_rows, const void* g,
                      int64_t ldg, int g_type, int64_t g_rows, const int64_t* src_idx,
                      const int64_t* dst_idx, const int64_t* seg_ptr, int64_t M, int K, int N, int R,
-                     float* gw, void* workspace, size_t workspace_bytes, void* stream);
+                     float* gw, float* gb, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

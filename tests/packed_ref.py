@@ -76,3 +76,16 @@ def weight_grad(a, g, bounds, src=None, dst=None):
         depth = parts * x.shape[0] + x.shape[0] // 128 + 2
         tol.append(2 * U * depth * 1.01 * (x.abs().t() @ y.abs()))
     return B(torch.stack(out), torch.stack(tol))
+
+
+def row_sums(g, bounds, dst=None, keep=None):
+    """[B [N]] per segment: sums of the rows of g (at most one rounding per row and chunk), rows with
+    ``keep`` False left out."""
+    out = []
+    for b, e in zip(bounds, bounds[1:]):
+        rows = torch.arange(b, e)
+        if keep is not None:
+            rows = rows[keep[b:e]]
+        y = g.double()[rows if dst is None else dst[rows]]
+        out.append(B(y.sum(0), U * (y.shape[0] + y.shape[0] // 128 + 2) * 1.01 * y.abs().sum(0)))
+    return out

@@ -67,7 +67,7 @@ def test_library_refuses_bad_arguments():
 
     def wgrad(codes=256, a_rows=10, g=256, g_type=0, g_rows=10, src=None, dst=None, seg=None, M=10, K=8, N=8, R=1, gw=256, ws=256,
               nbytes=need, ldg=8, fmt=0):
-        return lib.cxg_packed_wgrad(codes, 256, fmt, a_rows, g, ldg, g_type, g_rows, src, dst, seg, M, K, N, R, gw, ws, nbytes, None)
+        return lib.cxg_packed_wgrad(codes, 256, fmt, a_rows, g, ldg, g_type, g_rows, src, dst, seg, M, K, N, R, gw, None, ws, nbytes, None)
 
     for kw, status in ((dict(M=-1), -1), (dict(K=0), -1), (dict(N=0), -1), (dict(R=0), -1), (dict(R=2), -1), (dict(gw=None), -1),
                        (dict(codes=None), -1), (dict(codes=260), -1), (dict(g=None), -1), (dict(g=258), -1), (dict(a_rows=9), -1),
@@ -216,6 +216,32 @@ def test_weight_grad_rows_segments_and_maps(m, segs, maps):
     announce("packed_weight_grad %d rows, %d segments, maps %s" % (m, segs, maps))
     got = _wgrad(case, 60, "int8")
     check(got, packed_ref.weight_grad(case[2], case[3], case[4], case[5], case[6]), F32, "gw")
+
+
+@gpu
+@pytest.mark.parametrize("m,n", [(0, 5), (1, 3), (33, 1), (700, 47), (5000, 72), (1300, 300)])
+@pytest.mark.parametrize("k", [20, 140])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_row_sums_of_the_gradient(m, n, k, dtype):
+    """want_sums: the sums of the rows of g that count, per segment, beside the same weight gradient."""
+    import cxgnncomp
+    codes, exps, values, g, bounds, src, dst = _wgrad_case(m, k, n, dtype, segs=3, maps=m > 0, seed=m)
+    p = cxgnncomp.PackedRows(codes.cuda(), exps.cuda(), k)
+    maps = {}
+    keep = None
+    if m > 0:
+        src[::7] = -1
+        dst[3::11] = m
+        keep = (src >= 0) & (dst < m)
+        maps = dict(src_idx=src.cuda(), dst_idx=dst.cuda())
+    announce("packed_weight_grad sums %d x %d x %d %s" % (m, k, n, dtype))
+    gw, gb = cxgnncomp.packed_weight_grad(p, g.cuda(), torch.tensor(bounds).cuda(), want_sums=True, **maps)
+    assert tuple(gb.shape) == (3, n)
+    for r, want in enumerate(packed_ref.row_sums(g, bounds, dst, keep)):
+        check(gb[r], want, F32, "sums of segment %d" % r)
+    assert torch.equal(gw, cxgnncomp.packed_weight_grad(p, g.cuda(), torch.tensor(bounds).cuda(), **maps))
+    gw, gb = cxgnncomp.packed_weight_grad(p, g.cuda(), want_sums=True)
+    check(gb[0], packed_ref.row_sums(g, [0, m])[0], F32, "sums of all rows")
 
 
 @gpu
