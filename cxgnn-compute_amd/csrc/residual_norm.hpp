@@ -1,10 +1,9 @@
 // Shared by the forward and the backward kernel of the residual norm (see residual_norm_fwd.hip).
 #pragma once
-#include "row_types.hpp"
+#include "packed_rows.hpp"
 
 namespace cxg {
 
-constexpr int kRnThreads = 256;
 constexpr int kRnMaxCols = 8192;
 constexpr int kRnSums = 4;               // column sums of the backward pass
 
@@ -28,53 +27,127 @@ struct RnArgs {
   float* partial;                        // [blocks][kRnSums][cols]
 };
 
-// Team of L lanes that owns a row, ITEMS pieces of V values per lane: piece i of lane l starts at
-// column (i * L + l) * V, so that each load of a team is one contiguous run.
+// How the last piece of a row ends: with the row; short, its values then come from the V last columns; or
+// the whole row is shorter than one piece.
+enum RnTail { kRnWhole, kRnShort, kRnTiny };
+
+// A team of L lanes owns a row, PER columns per lane; narrow rows share a wave, wide ones take several
+// waves.  Piece i of lane l starts at column (i * L + l) * V: each load of a team is one contiguous run.
+template <typename TX, typename TF, int L_, int PER_, int TAIL_> struct RnTeam {
+  static constexpr int L = L_, PER = PER_, V = 16 / (sizeof(TX) > sizeof(TF) ? sizeof(TX) : sizeof(TF)), ITEMS = PER / V;
+  static constexpr int THREADS = L < 256 ? 256 : L, TEAMS = THREADS / L, WAVES = THREADS / CXG_WAVE;
+  static constexpr int TAIL = TAIL_;
+};
+
+// V values of a row from column c on, any alignment of the row; zeros where c is past its end.  A short
+// piece is read where it ends with the row, without a branch, and moved to its place by rn_widen.
+template <int TAIL, typename T, int V> __device__ __forceinline__ void rn_load(RowPiece<T, V>& p, const T* row, int c, int cols) {
+  if constexpr (TAIL == kRnTiny) {
+    p.load(row, c, cols);
+  } else {
+    p.t = (T)0.f;
+    if (c < cols) p.t = *reinterpret_cast<const typename RowPiece<T, V>::loose_t*>(row + (TAIL == kRnShort && c + V > cols ? cols - V : c));
+  }
+}
+template <int TAIL, typename T, int V> __device__ __forceinline__ void rn_widen(const RowPiece<T, V>& p, int c, int cols, float (&v)[V]) {
+  p.widen(v);
+  if constexpr (TAIL == kRnShort) {
+    if (c < cols && c + V > cols) {
+      const int s = c + V - cols;                        // 1 .. V - 1 values in front of the piece
+#pragma unroll
+      for (int k = V / 2; k >= 1; k /= 2)
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = (s & k) ? (j + k < V ? v[j + k] : 0.f) : v[j];
+    }
+  }
+}
+template <int TAIL, typename T, int V> __device__ __forceinline__ void rn_store(const float (&v)[V], T* row, int c, int cols) {
+  RowPiece<T, V> p;
+  p.narrow(v);
+  if constexpr (TAIL != kRnWhole) {
+    p.store(row, c, cols);
+  } else {
+    if (c < cols) *reinterpret_cast<typename RowPiece<T, V>::loose_t*>(row + c) = p.t;
+  }
+}
+
 template <int L, int V> __device__ __forceinline__ int rn_col(int item, int lane_in_team) {
   return (item * L + lane_in_team) * V;
 }
 
-// Sum over the team; every lane gets it.  L = 256: the four waves meet in LDS (`slot` alternates
-// between two buffers, so that one barrier per sum is enough).
-template <int L, int N>
-__device__ __forceinline__ void team_sum(float (&v)[N], float (*s_red)[kRnThreads / CXG_WAVE][2], int& slot) {
+// Sum over the team; every lane gets it.  Teams of several waves meet in LDS (`slot` alternates between
+// two buffers, so that one barrier per sum is enough).
+template <typename S, int N>
+__device__ __forceinline__ void team_sum(float (&v)[N], float (*s_red)[S::WAVES][2], int& slot) {
   static_assert(N <= 2, "two sums at most");
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = lanes_sum<(L < CXG_WAVE ? L : CXG_WAVE)>(v[i]);
-  if constexpr (L > CXG_WAVE) {
-    const int wave = threadIdx.x >> 6;
+  for (int i = 0; i < N; ++i) v[i] = lanes_sum<(S::L < CXG_WAVE ? S::L : CXG_WAVE)>(v[i]);
+  if constexpr (S::L > CXG_WAVE) {
+    constexpr int W = S::L / CXG_WAVE;                   // waves of a team
+    const int wave = threadIdx.x >> 6, first = wave / W * W;
     if (lane_id() == 0) {
 #pragma unroll
       for (int i = 0; i < N; ++i) s_red[slot][wave][i] = v[i];
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      v[i] = (s_red[slot][0][i] + s_red[slot][1][i]) + (s_red[slot][2][i] + s_red[slot][3][i]);
+    for (int i = 0; i < N; ++i) {
+      v[i] = s_red[slot][first][i];
+#pragma unroll
+      for (int w = 1; w < W; ++w) v[i] += s_red[slot][first + w][i];
+    }
     slot ^= 1;
   }
 }
 
-// fp32 parameter vectors: 0 (or `missing`) where there is no column or no vector
+// fp32 parameter vectors: 0 where there is no column, `missing` where there is no vector
 template <int L, int V, int ITEMS>
 __device__ __forceinline__ void rn_params(const float* p, int cols, int lit, float missing, float (&out)[ITEMS][V]) {
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = rn_col<L, V>(i, lit) + j;
-      out[i][j] = c < cols ? (p ? p[c] : missing) : 0.f;
+    for (int q = 0; q < V; q += 4) {
+      const int c = rn_col<L, V>(i, lit) + q;
+      RowPiece<float, 4> w;
+      if (p) {
+        w.load(p, c, cols);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w.t[j] = c + j < cols ? missing : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) out[i][q + j] = w.t[j];
     }
 }
 
+// F<TX, TF, L, PER, TAIL>(a, st) for the types and the width: 8 columns per lane (16 are no faster where
+// they fit) up to a team of 512 lanes.
+#define CXG_RN_WIDTH(F, TX, TF, TAIL)                                                      \
+  do {                                                                                     \
+    if (a.cols <= 32) return F<TX, TF, 4, 8, TAIL>(a, st);                                 \
+    if (a.cols <= 64) return F<TX, TF, 8, 8, TAIL>(a, st);                                 \
+    if (a.cols <= 128) return F<TX, TF, 16, 8, TAIL>(a, st);                               \
+    if (a.cols <= 256) return F<TX, TF, 32, 8, TAIL>(a, st);                               \
+    if (a.cols <= 512) return F<TX, TF, 64, 8, TAIL>(a, st);                               \
+    if (a.cols <= 1024) return F<TX, TF, 128, 8, TAIL>(a, st);                             \
+    if (a.cols <= 2048) return F<TX, TF, 256, 8, TAIL>(a, st);                             \
+    if (a.cols <= 4096) return F<TX, TF, 512, 8, TAIL>(a, st);                             \
+    return F<TX, TF, 512, 16, TAIL>(a, st);                                                \
+  } while (0)
+#define CXG_RN_TYPE(F, ST, TX, BT, TF)                                                     \
+  if (stream_type == ST && branch_type == BT) {                                            \
+    constexpr int V = 16 / (int)sizeof(TX);                                                \
+    if (a.cols % V == 0) CXG_RN_WIDTH(F, TX, TF, kRnWhole);                                \
+    if (a.cols > V) CXG_RN_WIDTH(F, TX, TF, kRnShort);                                     \
+    return F<TX, TF, 4, 8, kRnTiny>(a, st);                                                \
+  }
 #define CXG_RN_TYPES(F)                                                                    \
-  if (stream_type == CXG_F32 && branch_type == CXG_F32) return F<float, float>(a, vec, st);       \
-  if (stream_type == CXG_BF16 && branch_type == CXG_BF16) return F<bf16_t, bf16_t>(a, vec, st);   \
-  if (stream_type == CXG_F16 && branch_type == CXG_F16) return F<f16_t, f16_t>(a, vec, st);       \
-  if (stream_type == CXG_F32 && branch_type == CXG_BF16) return F<float, bf16_t>(a, vec, st);     \
-  if (stream_type == CXG_F32 && branch_type == CXG_F16) return F<float, f16_t>(a, vec, st);
+  CXG_RN_TYPE(F, CXG_F32, float, CXG_F32, float)                                           \
+  CXG_RN_TYPE(F, CXG_BF16, bf16_t, CXG_BF16, bf16_t)                                       \
+  CXG_RN_TYPE(F, CXG_F16, f16_t, CXG_F16, f16_t)                                           \
+  CXG_RN_TYPE(F, CXG_F32, float, CXG_BF16, bf16_t)                                         \
+  CXG_RN_TYPE(F, CXG_F32, float, CXG_F16, f16_t)
 
 int rn_check(const RnArgs& a, int stream_type, int branch_type);
-bool rn_aligned(const void* p, int64_t ld, size_t bytes, int v);
 
 }  // namespace cxg

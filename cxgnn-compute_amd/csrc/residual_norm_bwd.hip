@@ -22,12 +22,12 @@
 namespace cxg {
 namespace {
 
-constexpr int kRnMaxBlocks = 1024;       // partial rows
+constexpr int kRnMaxBlocks = 768;        // partial rows; three blocks of 256 threads per CU are resident
 
-template <typename TX, typename TF, int V, int L, int ITEMS>
-__global__ __launch_bounds__(kRnThreads) void residual_norm_bwd_kernel(RnArgs a) {
-  __shared__ float s_red[2][kRnThreads / CXG_WAVE][2];
-  constexpr int kTeams = kRnThreads / L;
+template <typename TX, typename TF, typename S>
+__global__ __launch_bounds__(S::THREADS) void residual_norm_bwd_kernel(RnArgs a) {
+  constexpr int L = S::L, V = S::V, ITEMS = S::ITEMS, kTeams = S::TEAMS;
+  __shared__ float s_red[2][S::WAVES][2];
   const int lit = threadIdx.x % L, team = threadIdx.x / L;
   const int cols = a.cols;
   const float inv_c = 1.0f / (float)cols;
@@ -40,39 +40,33 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_bwd_kernel(RnArgs a)
   rn_params<L, V, ITEMS>(post ? a.post_b : nullptr, cols, lit, 0.f, b1);
   rn_params<L, V, ITEMS>(pre ? a.pre_w : nullptr, cols, lit, 1.f, w2);
   rn_params<L, V, ITEMS>(a.gate_kind == CXG_GATE_CHANNEL ? static_cast<const float*>(a.gate) : nullptr, cols, lit, 1.f, gc);
-  bool in[ITEMS];
+  auto inside = [&](int i, int j) { return rn_col<L, V>(i, lit) + (S::TAIL != kRnWhole ? j : 0) < cols; };
   float sums[kRnSums][ITEMS][V];
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
-    in[i] = rn_col<L, V>(i, lit) < cols;
+  for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
     for (int q = 0; q < kRnSums; ++q)
 #pragma unroll
       for (int j = 0; j < V; ++j) sums[q][i][j] = 0.f;
-  }
 
   for (int64_t base = (int64_t)blockIdx.x * kTeams; base < a.rows; base += (int64_t)gridDim.x * kTeams) {
     const int64_t row = base + team;
     const bool live = row < a.rows;
     const int64_t rr = live ? row : 0;
-    Piece<TX, V> px[ITEMS], pdr[ITEMS];
-    Piece<TF, V> pf[ITEMS], pg[ITEMS], pdy[ITEMS];
-    const TX* const xrow = static_cast<const TX*>(a.x) + rr * a.ldx;
-    const TF* const frow = static_cast<const TF*>(a.f) + rr * a.ldf;
-    const TX* const drrow = static_cast<const TX*>(a.dr) + rr * a.lddr;
-    const TF* const dyrow = static_cast<const TF*>(a.dy) + rr * a.lddy;
+    RowPiece<TX, V> px[ITEMS], pdr[ITEMS];
+    RowPiece<TF, V> pf[ITEMS], pg[ITEMS], pdy[ITEMS];
     const bool full = a.gate_kind == CXG_GATE_FULL;
+    const int here = live ? cols : 0;                     // a row that does not exist adds zeros everywhere
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      px[i].clear(); pf[i].clear(); pdr[i].clear(); pdy[i].clear(); pg[i].clear();
-      if (in[i] && live) {                              // a row that does not exist adds zeros everywhere
-        const int c = rn_col<L, V>(i, lit);
-        px[i].load(xrow + c);
-        if (a.f) pf[i].load(frow + c);
-        if (a.dr) pdr[i].load(drrow + c);
-        if (a.dy) pdy[i].load(dyrow + c);
-        if (full) pg[i].load(static_cast<const TF*>(a.gate) + rr * a.ldg + c);
-      }
+      const int c = rn_col<L, V>(i, lit);
+      px[i].t = pdr[i].t = (TX)0.f;
+      pf[i].t = pg[i].t = pdy[i].t = (TF)0.f;
+      rn_load<S::TAIL>(px[i], static_cast<const TX*>(a.x) + rr * a.ldx, c, here);
+      if (a.f) rn_load<S::TAIL>(pf[i], static_cast<const TF*>(a.f) + rr * a.ldf, c, here);
+      if (a.dr) rn_load<S::TAIL>(pdr[i], static_cast<const TX*>(a.dr) + rr * a.lddr, c, here);
+      if (a.dy) rn_load<S::TAIL>(pdy[i], static_cast<const TF*>(a.dy) + rr * a.lddy, c, here);
+      if (full) rn_load<S::TAIL>(pg[i], static_cast<const TF*>(a.gate) + rr * a.ldg, c, here);
     }
     const float grow = a.gate_kind == CXG_GATE_ROW && live ? (float)static_cast<const TF*>(a.gate)[rr * a.ldg] : 1.f;
     float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
@@ -83,7 +77,12 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_bwd_kernel(RnArgs a)
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       float x[V], f[V], dy[V], gf[V];
-      px[i].widen(x); pf[i].widen(f); pdy[i].widen(dy); pg[i].widen(gf); pdr[i].widen(g[i]);
+      const int c = rn_col<L, V>(i, lit);
+      rn_widen<S::TAIL>(px[i], c, cols, x);
+      rn_widen<S::TAIL>(pf[i], c, cols, f);
+      rn_widen<S::TAIL>(pdy[i], c, cols, dy);
+      rn_widen<S::TAIL>(pg[i], c, cols, gf);
+      rn_widen<S::TAIL>(pdr[i], c, cols, g[i]);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         fh[i][j] = post ? (f[j] - st.x) * st.y : f[j];
@@ -100,12 +99,12 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_bwd_kernel(RnArgs a)
       }
     }
     if (pre) {
-      team_sum<L, 2>(s, s_red, slot);
+      team_sum<S, 2>(s, s_red, slot);
       const float m0 = pre_layer ? s[0] * inv_c : 0.f, m1 = s[1] * inv_c;
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
         float dy[V];
-        pdy[i].widen(dy);
+        rn_widen<S::TAIL>(pdy[i], rn_col<L, V>(i, lit), cols, dy);
 #pragma unroll
         for (int j = 0; j < V; ++j) g[i][j] += st.w * (dy[j] * w2[i][j] - m0 - rh[i][j] * m1);
       }
@@ -113,38 +112,32 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_bwd_kernel(RnArgs a)
     if (a.dx && live) {
       TX* const out = static_cast<TX*>(a.dx) + rr * cols;
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i)
-        if (in[i]) {
-          float o[V];
+      for (int i = 0; i < ITEMS; ++i) {
+        float o[V];
 #pragma unroll
-          for (int j = 0; j < V; ++j) o[j] = a.res_scale * g[i][j];
-          Piece<TX, V> p;
-          p.narrow(o);
-          p.store(out + rn_col<L, V>(i, lit));
-        }
+        for (int j = 0; j < V; ++j) o[j] = a.res_scale * g[i][j];
+        rn_store<S::TAIL>(o, out, rn_col<L, V>(i, lit), cols);
+      }
     }
     if (a.dgate) {
       if (full) {
         if (live) {
           TF* const out = static_cast<TF*>(a.dgate) + rr * cols;
 #pragma unroll
-          for (int i = 0; i < ITEMS; ++i)
-            if (in[i]) {
-              float o[V];
+          for (int i = 0; i < ITEMS; ++i) {
+            float o[V];
 #pragma unroll
-              for (int j = 0; j < V; ++j) o[j] = a.branch_scale * g[i][j] * h[i][j];
-              Piece<TF, V> p;
-              p.narrow(o);
-              p.store(out + rn_col<L, V>(i, lit));
-            }
+            for (int j = 0; j < V; ++j) o[j] = a.branch_scale * g[i][j] * h[i][j];
+            rn_store<S::TAIL>(o, out, rn_col<L, V>(i, lit), cols);
+          }
         }
       } else if (a.gate_kind == CXG_GATE_ROW) {
         float d[1] = {0.f};
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-          for (int j = 0; j < V; ++j) d[0] += in[i] ? g[i][j] * h[i][j] : 0.f;
-        team_sum<L, 1>(d, s_red, slot);
+          for (int j = 0; j < V; ++j) d[0] += inside(i, j) ? g[i][j] * h[i][j] : 0.f;
+        team_sum<S, 1>(d, s_red, slot);
         if (live && lit == 0) static_cast<TF*>(a.dgate)[rr] = (TF)(a.branch_scale * d[0]);
       }
     }
@@ -164,22 +157,19 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_bwd_kernel(RnArgs a)
       if (a.df) {
         float m0 = 0.f, m1 = 0.f;
         if (post) {
-          team_sum<L, 2>(q, s_red, slot);
+          team_sum<S, 2>(q, s_red, slot);
           m0 = post_layer ? q[0] * inv_c : 0.f;
           m1 = q[1] * inv_c;
         }
         if (live) {
           TF* const out = static_cast<TF*>(a.df) + rr * cols;
 #pragma unroll
-          for (int i = 0; i < ITEMS; ++i)
-            if (in[i]) {
-              float o[V];
+          for (int i = 0; i < ITEMS; ++i) {
+            float o[V];
 #pragma unroll
-              for (int j = 0; j < V; ++j) o[j] = post ? st.y * (g[i][j] - m0 - fh[i][j] * m1) : g[i][j];
-              Piece<TF, V> p;
-              p.narrow(o);
-              p.store(out + rn_col<L, V>(i, lit));
-            }
+            for (int j = 0; j < V; ++j) o[j] = post ? st.y * (g[i][j] - m0 - fh[i][j] * m1) : g[i][j];
+            rn_store<S::TAIL>(o, out, rn_col<L, V>(i, lit), cols);
+          }
         }
       }
     }
@@ -188,7 +178,7 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_bwd_kernel(RnArgs a)
   // the block's partial row: teams of a wave in registers, waves in LDS
   if (a.partial == nullptr) return;
   float* const out = a.partial + (size_t)blockIdx.x * kRnSums * cols;
-  if constexpr (L >= kRnThreads) {
+  if constexpr (kTeams == 1) {
 #pragma unroll
     for (int q = 0; q < kRnSums; ++q)
 #pragma unroll
@@ -199,8 +189,9 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_bwd_kernel(RnArgs a)
           if (c < cols) out[(size_t)q * cols + c] = sums[q][i][j];
         }
   } else {
-    constexpr int kWaves = kRnThreads / CXG_WAVE, kWidth = L * V * ITEMS;
-    __shared__ float s_col[kWaves][kWidth];
+    constexpr int kParts = L < CXG_WAVE ? S::WAVES : kTeams;     // waves, or teams of whole waves
+    __shared__ float s_col[kParts][L * S::PER];
+    const int part = L < CXG_WAVE ? (int)(threadIdx.x >> 6) : team;
 #pragma unroll
     for (int q = 0; q < kRnSums; ++q) {
       if (q) __syncthreads();
@@ -209,11 +200,15 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_bwd_kernel(RnArgs a)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const float t = groups_sum<L>(sums[q][i][j]);
-          if ((threadIdx.x & (CXG_WAVE - 1)) < L) s_col[threadIdx.x >> 6][rn_col<L, V>(i, lit) + j] = t;
+          if (L >= CXG_WAVE || (int)(threadIdx.x & (CXG_WAVE - 1)) < L) s_col[part][rn_col<L, V>(i, lit) + j] = t;
         }
       __syncthreads();
-      for (int c = threadIdx.x; c < cols; c += kRnThreads)
-        out[(size_t)q * cols + c] = (s_col[0][c] + s_col[1][c]) + (s_col[2][c] + s_col[3][c]);
+      for (int c = threadIdx.x; c < cols; c += S::THREADS) {
+        float t = s_col[0][c];
+#pragma unroll
+        for (int k = 1; k < kParts; ++k) t += s_col[k][c];
+        out[(size_t)q * cols + c] = t;
+      }
     }
   }
 }
@@ -264,43 +259,23 @@ __global__ __launch_bounds__(kFinThreads) void residual_norm_sums_kernel(RnFinal
   if (a.dgate) a.dgate[c] = a.branch_scale * (w * s2 + b * s3);
 }
 
-int64_t bwd_blocks(int64_t rows, int teams) {
-  const int64_t blocks = ceil_div(rows, (int64_t)teams);
-  return blocks > kRnMaxBlocks ? kRnMaxBlocks : blocks;
+// Blocks of the row kernel: what is resident (one block of 512 threads per CU), each walks its rows.
+int64_t bwd_blocks(int64_t rows, int teams, int threads) {
+  const int64_t blocks = ceil_div(rows, (int64_t)teams), most = threads > 256 ? 256 : kRnMaxBlocks;
+  return blocks > most ? most : blocks;
 }
 
 // launches the row kernel; returns the number of partial rows, or a negative status
-template <typename TX, typename TF, int V, int L, int ITEMS> int launch_bwd(const RnArgs& a, hipStream_t st) {
-  const int64_t blocks = bwd_blocks(a.rows, kRnThreads / L);
-  hipLaunchKernelGGL((residual_norm_bwd_kernel<TX, TF, V, L, ITEMS>), dim3((unsigned)blocks), dim3(kRnThreads), 0, st, a);
+template <typename TX, typename TF, int L, int PER, int TAIL> int launch_bwd(const RnArgs& a, hipStream_t st) {
+  typedef RnTeam<TX, TF, L, PER, TAIL> S;
+  const int64_t blocks = bwd_blocks(a.rows, S::TEAMS, S::THREADS);
+  hipLaunchKernelGGL((residual_norm_bwd_kernel<TX, TF, S>), dim3((unsigned)blocks), dim3(S::THREADS), 0, st, a);
   CXG_LAUNCH_CHECK("residual_norm_bwd_kernel");
   return (int)blocks;
 }
 
-template <typename TX, typename TF> int dispatch_bwd(const RnArgs& a, bool vec, hipStream_t st) {
-  constexpr int W = 16 / (sizeof(TX) > sizeof(TF) ? sizeof(TX) : sizeof(TF));
-  const int n = vec ? a.cols / W : a.cols;
-  if (vec) {
-    if (n <= 8) return launch_bwd<TX, TF, W, 8, 1>(a, st);
-    if (n <= 16) return launch_bwd<TX, TF, W, 8, 2>(a, st);
-    if (n <= 32) return launch_bwd<TX, TF, W, 16, 2>(a, st);
-    if (n <= 64) return launch_bwd<TX, TF, W, 32, 2>(a, st);
-    if (n <= 128) return launch_bwd<TX, TF, W, 64, 2>(a, st);
-    if (n <= 512) return launch_bwd<TX, TF, W, 256, 2>(a, st);
-    if (n <= 1024) return launch_bwd<TX, TF, W, 256, 4>(a, st);
-    if constexpr (W == 4) return launch_bwd<TX, TF, W, 256, 8>(a, st);
-  } else {
-    if (n <= 16) return launch_bwd<TX, TF, 1, 8, 2>(a, st);
-    if (n <= 64) return launch_bwd<TX, TF, 1, 16, 4>(a, st);
-    if (n <= 256) return launch_bwd<TX, TF, 1, 64, 4>(a, st);
-    if (n <= 1024) return launch_bwd<TX, TF, 1, 256, 4>(a, st);
-    return launch_bwd<TX, TF, 1, 256, 32>(a, st);
-  }
-  return set_error(CXG_ERR_UNSUPPORTED, "rows of more than %d columns", kRnMaxCols);
-}
-
-int dispatch_bwd_types(const RnArgs& a, int stream_type, int branch_type, bool vec, hipStream_t st) {
-  CXG_RN_TYPES(dispatch_bwd)
+int dispatch_bwd(const RnArgs& a, int stream_type, int branch_type, hipStream_t st) {
+  CXG_RN_TYPES(launch_bwd)
   return set_error(CXG_ERR_UNSUPPORTED, "unsupported types");
 }
 
@@ -311,7 +286,7 @@ extern "C" {
 
 size_t cxg_residual_norm_workspace_bytes(int64_t rows, int cols) {
   if (rows < 0 || cols < 1) return 0;
-  return (size_t)cxg::bwd_blocks(rows, 1) * cxg::kRnSums * (size_t)cols * sizeof(float) + 256;
+  return (size_t)cxg::bwd_blocks(rows, 1, 256) * cxg::kRnSums * (size_t)cols * sizeof(float) + 256;
 }
 
 int cxg_residual_norm_bwd(const void* x, int64_t ldx, const void* f, int64_t ldf, const void* gate, int64_t ldg,
@@ -354,13 +329,7 @@ int cxg_residual_norm_bwd(const void* x, int64_t ldx, const void* f, int64_t ldf
   }
   if (!channel) a.dgate = dgate;
   if (rows > 0) {
-    const size_t sx = value_bytes(stream_type), sf = value_bytes(branch_type);
-    const int v = stream_type == CXG_F32 || branch_type == CXG_F32 ? 4 : 8;
-    const bool full = gate_kind == CXG_GATE_FULL;
-    const bool vec = cols % v == 0 && rn_aligned(x, ldx, sx, v) && rn_aligned(f, ldf, sf, v) && rn_aligned(dr, lddr, sx, v) &&
-                     rn_aligned(dy, lddy, sf, v) && rn_aligned(dx, 0, sx, v) && rn_aligned(df, 0, sf, v) &&
-                     (!full || (rn_aligned(gate, ldg, sf, v) && rn_aligned(dgate, 0, sf, v)));
-    const int blocks = dispatch_bwd_types(a, stream_type, branch_type, vec, st);
+    const int blocks = dispatch_bwd(a, stream_type, branch_type, st);
     if (blocks < 0) return blocks;
     fin.blocks = blocks;
   }

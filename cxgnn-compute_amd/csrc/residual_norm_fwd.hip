@@ -11,9 +11,11 @@
 //
 // Bound: memory.  A row is read once (x, f), kept in registers through both norms and written once
 // (r, y); everything else are the reductions over its columns: mean first, then the sum of squared
-// deviations from the registers, so a mean far from zero costs no digits.  A team of L lanes owns a
-// row, up to four 16-byte pieces per lane: narrow rows share a wave (8 lanes for 128 fp32 columns,
-// whose reductions are three data-parallel moves each), rows beyond 64 lanes take a block.
+// deviations from the registers, so a mean far from zero costs no digits.  A team of lanes owns a row,
+// 8 columns per lane whatever the width: the vectors of the norms then stay in registers from row to row
+// and enough waves fit a CU to keep memory busy.  (Up to 32 columns per lane left rows of 512 bf16 columns
+// at 1.2 TB/s; a grid of more blocks than are resident loads the vectors more often, 3.6 against 5.1 TB/s.)  Rows start at any value: the 16-byte
+// accesses assume the alignment of one value only.
 #include "residual_norm.hpp"
 
 namespace cxg {
@@ -31,21 +33,21 @@ int rn_check(const RnArgs& a, int stream_type, int branch_type) {
   CXG_REQUIRE(a.f || a.rows == 0 || (a.gate_kind == CXG_GATE_NONE && a.post_kind == CXG_NORM_NONE), CXG_ERR_ARG,
               "a gate or a norm of the branch needs branch rows");
   CXG_REQUIRE(a.rows == 0 || a.x, CXG_ERR_ARG, "null x");
+  const uintptr_t sx = value_bytes(stream_type) - 1, sf = value_bytes(branch_type) - 1;
+  CXG_REQUIRE((((uintptr_t)a.x | (uintptr_t)a.r | (uintptr_t)a.dr | (uintptr_t)a.dx) & sx) == 0 &&
+                  (((uintptr_t)a.f | (uintptr_t)a.y | (uintptr_t)a.dy | (uintptr_t)a.df) & sf) == 0 &&
+                  ((uintptr_t)a.gate & (a.gate_kind == CXG_GATE_CHANNEL ? 3 : sf)) == 0,
+              CXG_ERR_ARG, "rows that are not aligned to their values");
   CXG_REQUIRE(a.ldx >= 0 && a.ldf >= 0 && a.ldg >= 0 && a.lddr >= 0 && a.lddy >= 0, CXG_ERR_ARG, "negative row stride");
   return CXG_OK;
 }
 
-// Whether pieces of v values can be read at every row.
-bool rn_aligned(const void* p, int64_t ld, size_t bytes, int v) {
-  return p == nullptr || (((uintptr_t)p & (bytes * v - 1)) == 0 && ld % v == 0);
-}
-
 namespace {
 
-template <typename TX, typename TF, int V, int L, int ITEMS>
-__global__ __launch_bounds__(kRnThreads) void residual_norm_fwd_kernel(RnArgs a) {
-  __shared__ float s_red[2][kRnThreads / CXG_WAVE][2];
-  constexpr int kTeams = kRnThreads / L;
+template <typename TX, typename TF, typename S>
+__global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a) {
+  constexpr int L = S::L, V = S::V, ITEMS = S::ITEMS, kTeams = S::TEAMS;
+  __shared__ float s_red[2][S::WAVES][2];
   const int lit = threadIdx.x % L, team = threadIdx.x / L;
   const int cols = a.cols;
   const float inv_c = 1.0f / (float)cols;
@@ -60,39 +62,28 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_fwd_kernel(RnArgs a)
     rn_params<L, V, ITEMS>(a.pre_b, cols, lit, 0.f, b2);
   }
   if (a.gate_kind == CXG_GATE_CHANNEL) rn_params<L, V, ITEMS>(static_cast<const float*>(a.gate), cols, lit, 1.f, gc);
-  bool in[ITEMS];
-#pragma unroll
-  for (int i = 0; i < ITEMS; ++i) in[i] = rn_col<L, V>(i, lit) < cols;
+  auto inside = [&](int i, int j) { return rn_col<L, V>(i, lit) + (S::TAIL != kRnWhole ? j : 0) < cols; };
 
   // every lane stays in the loop as long as its block: the reductions need whole waves
   for (int64_t base = (int64_t)blockIdx.x * kTeams; base < a.rows; base += (int64_t)gridDim.x * kTeams) {
     const int64_t row = base + team;
     const bool live = row < a.rows;
     const int64_t rr = live ? row : 0;
-    Piece<TX, V> px[ITEMS];
-    Piece<TF, V> pf[ITEMS], pg[ITEMS];
+    RowPiece<TX, V> px[ITEMS];
+    RowPiece<TF, V> pf[ITEMS], pg[ITEMS];
     const TX* const xrow = static_cast<const TX*>(a.x) + rr * a.ldx;
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      px[i].clear();
-      if (in[i]) px[i].load(xrow + rn_col<L, V>(i, lit));
-    }
+    for (int i = 0; i < ITEMS; ++i) rn_load<S::TAIL>(px[i], xrow, rn_col<L, V>(i, lit), cols);
     if (a.f) {
       const TF* const frow = static_cast<const TF*>(a.f) + rr * a.ldf;
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i) {
-        pf[i].clear();
-        if (in[i]) pf[i].load(frow + rn_col<L, V>(i, lit));
-      }
+      for (int i = 0; i < ITEMS; ++i) rn_load<S::TAIL>(pf[i], frow, rn_col<L, V>(i, lit), cols);
     }
     float grow = 1.f;
     if (a.gate_kind == CXG_GATE_FULL) {
       const TF* const gr = static_cast<const TF*>(a.gate) + rr * a.ldg;
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i) {
-        pg[i].clear();
-        if (in[i]) pg[i].load(gr + rn_col<L, V>(i, lit));
-      }
+      for (int i = 0; i < ITEMS; ++i) rn_load<S::TAIL>(pg[i], gr, rn_col<L, V>(i, lit), cols);
     } else if (a.gate_kind == CXG_GATE_ROW) {
       grow = (float)static_cast<const TF*>(a.gate)[rr * a.ldg];
     }
@@ -101,7 +92,7 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_fwd_kernel(RnArgs a)
     float mean1 = 0.f, rstd1 = 1.f, mean2 = 0.f, rstd2 = 1.f;
     if (a.f) {
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i) pf[i].widen(v[i]);
+      for (int i = 0; i < ITEMS; ++i) rn_widen<S::TAIL>(pf[i], rn_col<L, V>(i, lit), cols, v[i]);
       if (a.post_kind != CXG_NORM_NONE) {
         float s[1];
         if (a.post_kind == CXG_NORM_LAYER) {
@@ -110,7 +101,7 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_fwd_kernel(RnArgs a)
           for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
             for (int j = 0; j < V; ++j) s[0] += v[i][j];
-          team_sum<L, 1>(s, s_red, slot);
+          team_sum<S, 1>(s, s_red, slot);
           mean1 = s[0] * inv_c;
         }
         s[0] = 0.f;
@@ -118,10 +109,10 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_fwd_kernel(RnArgs a)
         for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            v[i][j] = in[i] ? v[i][j] - mean1 : 0.f;
+            v[i][j] = inside(i, j) ? v[i][j] - mean1 : 0.f;
             s[0] += v[i][j] * v[i][j];
           }
-        team_sum<L, 1>(s, s_red, slot);
+        team_sum<S, 1>(s, s_red, slot);
         rstd1 = 1.0f / sqrtf(s[0] * inv_c + a.eps);
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
@@ -133,7 +124,7 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_fwd_kernel(RnArgs a)
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
           float g[V];
-          pg[i].widen(g);
+          rn_widen<S::TAIL>(pg[i], rn_col<L, V>(i, lit), cols, g);
 #pragma unroll
           for (int j = 0; j < V; ++j) v[i][j] *= g[j];
         }
@@ -146,7 +137,7 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_fwd_kernel(RnArgs a)
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
         float x[V];
-        px[i].widen(x);
+        rn_widen<S::TAIL>(px[i], rn_col<L, V>(i, lit), cols, x);
 #pragma unroll
         for (int j = 0; j < V; ++j) v[i][j] = a.res_scale * x[j] + bs * v[i][j];
       }
@@ -154,7 +145,7 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_fwd_kernel(RnArgs a)
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
         float x[V];
-        px[i].widen(x);
+        rn_widen<S::TAIL>(px[i], rn_col<L, V>(i, lit), cols, x);
 #pragma unroll
         for (int j = 0; j < V; ++j) v[i][j] = a.res_scale * x[j];
       }
@@ -162,12 +153,7 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_fwd_kernel(RnArgs a)
     if (a.r && live) {
       TX* const out = static_cast<TX*>(a.r) + rr * cols;
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i)
-        if (in[i]) {
-          Piece<TX, V> p;
-          p.narrow(v[i]);
-          p.store(out + rn_col<L, V>(i, lit));
-        }
+      for (int i = 0; i < ITEMS; ++i) rn_store<S::TAIL>(v[i], out, rn_col<L, V>(i, lit), cols);
     }
     if (a.pre_kind != CXG_NORM_NONE) {
       float s[1];
@@ -177,7 +163,7 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_fwd_kernel(RnArgs a)
         for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
           for (int j = 0; j < V; ++j) s[0] += v[i][j];
-        team_sum<L, 1>(s, s_red, slot);
+        team_sum<S, 1>(s, s_red, slot);
         mean2 = s[0] * inv_c;
       }
       s[0] = 0.f;
@@ -185,23 +171,20 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_fwd_kernel(RnArgs a)
       for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          v[i][j] = in[i] ? v[i][j] - mean2 : 0.f;
+          v[i][j] = inside(i, j) ? v[i][j] - mean2 : 0.f;
           s[0] += v[i][j] * v[i][j];
         }
-      team_sum<L, 1>(s, s_red, slot);
+      team_sum<S, 1>(s, s_red, slot);
       rstd2 = 1.0f / sqrtf(s[0] * inv_c + a.eps);
       if (live) {
         TF* const out = static_cast<TF*>(a.y) + rr * cols;
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-          if (in[i]) {
-            float o[V];
+        for (int i = 0; i < ITEMS; ++i) {
+          float o[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) o[j] = v[i][j] * rstd2 * w2[i][j] + b2[i][j];
-            Piece<TF, V> p;
-            p.narrow(o);
-            p.store(out + rn_col<L, V>(i, lit));
-          }
+          for (int j = 0; j < V; ++j) o[j] = v[i][j] * rstd2 * w2[i][j] + b2[i][j];
+          rn_store<S::TAIL>(o, out, rn_col<L, V>(i, lit), cols);
+        }
       }
     }
     if (a.stats && live && lit == 0)
@@ -209,35 +192,13 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_fwd_kernel(RnArgs a)
   }
 }
 
-template <typename TX, typename TF, int V, int L, int ITEMS> int launch_fwd(const RnArgs& a, hipStream_t st) {
-  constexpr int kTeams = kRnThreads / L;
-  int64_t blocks = ceil_div(a.rows, (int64_t)kTeams);
-  if (blocks > 256 * 16) blocks = 256 * 16;
-  hipLaunchKernelGGL((residual_norm_fwd_kernel<TX, TF, V, L, ITEMS>), dim3((unsigned)blocks), dim3(kRnThreads), 0, st, a);
+template <typename TX, typename TF, int L, int PER, int TAIL> int launch_fwd(const RnArgs& a, hipStream_t st) {
+  typedef RnTeam<TX, TF, L, PER, TAIL> S;
+  int64_t blocks = ceil_div(a.rows, (int64_t)S::TEAMS);
+  if (blocks > 256 * 5) blocks = 256 * 5;                // what is resident: a block loads the vectors once
+  hipLaunchKernelGGL((residual_norm_fwd_kernel<TX, TF, S>), dim3((unsigned)blocks), dim3(S::THREADS), 0, st, a);
   CXG_LAUNCH_CHECK("residual_norm_fwd_kernel");
   return CXG_OK;
-}
-
-template <typename TX, typename TF> int dispatch_fwd(const RnArgs& a, bool vec, hipStream_t st) {
-  constexpr int W = 16 / (sizeof(TX) > sizeof(TF) ? sizeof(TX) : sizeof(TF));
-  const int n = vec ? a.cols / W : a.cols;                  // pieces of a row
-  if (vec) {
-    if (n <= 8) return launch_fwd<TX, TF, W, 8, 1>(a, st);
-    if (n <= 16) return launch_fwd<TX, TF, W, 8, 2>(a, st);
-    if (n <= 32) return launch_fwd<TX, TF, W, 8, 4>(a, st);
-    if (n <= 64) return launch_fwd<TX, TF, W, 16, 4>(a, st);
-    if (n <= 128) return launch_fwd<TX, TF, W, 32, 4>(a, st);
-    if (n <= 256) return launch_fwd<TX, TF, W, 64, 4>(a, st);
-    if (n <= 1024) return launch_fwd<TX, TF, W, 256, 4>(a, st);
-    if constexpr (W == 4) return launch_fwd<TX, TF, W, 256, 8>(a, st);
-  } else {
-    if (n <= 16) return launch_fwd<TX, TF, 1, 8, 2>(a, st);
-    if (n <= 64) return launch_fwd<TX, TF, 1, 16, 4>(a, st);
-    if (n <= 256) return launch_fwd<TX, TF, 1, 64, 4>(a, st);
-    if (n <= 1024) return launch_fwd<TX, TF, 1, 256, 4>(a, st);
-    return launch_fwd<TX, TF, 1, 256, 32>(a, st);
-  }
-  return set_error(CXG_ERR_UNSUPPORTED, "rows of more than %d columns", kRnMaxCols);
 }
 
 }  // namespace
@@ -261,12 +222,7 @@ extern "C" int cxg_residual_norm_fwd(const void* x, int64_t ldx, const void* f, 
   CXG_REQUIRE(rows == 0 || r || (pre_kind != CXG_NORM_NONE && !f), CXG_ERR_ARG, "null r");
   CXG_REQUIRE(((uintptr_t)stats & 15) == 0, CXG_ERR_ARG, "stats must be 16-byte aligned");
   if (rows == 0) return CXG_OK;
-  const size_t sx = value_bytes(stream_type), sf = value_bytes(branch_type);
-  const int v = stream_type == CXG_F32 || branch_type == CXG_F32 ? 4 : 8;
-  const bool vec = cols % v == 0 && rn_aligned(x, ldx, sx, v) && rn_aligned(f, ldf, sf, v) &&
-                   (gate_kind != CXG_GATE_FULL || rn_aligned(gate, ldg, sf, v)) && rn_aligned(r, 0, sx, v) &&
-                   rn_aligned(y, 0, sf, v);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  CXG_RN_TYPES(dispatch_fwd)
+  CXG_RN_TYPES(launch_fwd)
   return set_error(CXG_ERR_UNSUPPORTED, "unsupported types");
 }

@@ -1,5 +1,4 @@
-// Rows of fp32, bf16 or fp16 values as vectors of floats: loads widen exactly, stores round to the
-// nearest value of the type (ties to even).
+// Value types of rows that may be narrower than fp32, and sums across lanes.
 #pragma once
 #include "cxg_common.hpp"
 
@@ -7,46 +6,6 @@ namespace cxg {
 
 typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
-
-template <int BYTES> struct RawBits;
-template <> struct RawBits<2> { typedef uint16_t type; };
-template <> struct RawBits<4> { typedef uint32_t type; };
-template <> struct RawBits<8> { typedef uint32_t type __attribute__((ext_vector_type(2))); };
-template <> struct RawBits<16> { typedef uint32_t type __attribute__((ext_vector_type(4))); };
-
-// V consecutive values as they lie in memory: at most 16 bytes, one load
-template <typename T, int V> struct Piece {
-  static_assert(sizeof(T) * V <= 16, "one load");
-  typedef typename RawBits<(int)sizeof(T) * V>::type bits_t;
-  typedef T vec_t __attribute__((ext_vector_type(V)));
-  bits_t bits;
-  __device__ __forceinline__ void load(const T* p) { bits = *reinterpret_cast<const bits_t*>(p); }
-  __device__ __forceinline__ void clear() { bits = bits_t{}; }
-  __device__ __forceinline__ void widen(float (&v)[V]) const {
-    const vec_t t = __builtin_bit_cast(vec_t, bits);
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = (float)t[i];
-  }
-  __device__ __forceinline__ void narrow(const float (&v)[V]) {
-    vec_t t;
-#pragma unroll
-    for (int i = 0; i < V; ++i) t[i] = (T)v[i];
-    bits = __builtin_bit_cast(bits_t, t);
-  }
-  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<bits_t*>(p) = bits; }
-  __device__ __forceinline__ void store_streaming(T* p) const {
-    __builtin_nontemporal_store(bits, reinterpret_cast<bits_t*>(p));
-  }
-};
-template <typename T> struct Piece<T, 1> {
-  T t;
-  __device__ __forceinline__ void load(const T* p) { t = *p; }
-  __device__ __forceinline__ void clear() { t = (T)0.f; }
-  __device__ __forceinline__ void widen(float (&v)[1]) const { v[0] = (float)t; }
-  __device__ __forceinline__ void narrow(const float (&v)[1]) { t = (T)v[0]; }
-  __device__ __forceinline__ void store(T* p) const { *p = t; }
-  __device__ __forceinline__ void store_streaming(T* p) const { *p = t; }
-};
 
 inline size_t value_bytes(int type) { return type == CXG_F32 ? 4 : 2; }
 inline bool value_type_ok(int type) { return type == CXG_F32 || type == CXG_BF16 || type == CXG_F16; }
@@ -81,7 +40,8 @@ template <int L> __device__ __forceinline__ float lanes_sum(float v) {
 // Sum over the lanes l, l + L, l + 2L, ... of the wave (same position in every group of L lanes).
 template <int L> __device__ __forceinline__ float groups_sum(float v) {
   typedef unsigned v2u __attribute__((ext_vector_type(2)));
-  static_assert(L >= 8, "groups of at least eight lanes");
+  static_assert(L >= 4, "groups of at least four lanes");
+  if constexpr (L <= 4) v += __shfl_xor(v, 4, CXG_WAVE);
   if constexpr (L <= 8) v += __shfl_xor(v, 8, CXG_WAVE);
   if constexpr (L <= 16) {
     const v2u r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);

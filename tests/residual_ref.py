@@ -4,7 +4,7 @@ import torch
 from rounding import B, const
 
 ROW_DEPTH = 64          # additions on the longest path of a sum over a row: 32 per lane, 6 + 2 across lanes and waves
-COL_DEPTH = 160         # ... over up to 4096 rows: 4096 / 1024 per team, 3 + 2 in a block, 64 + 15 partial rows
+COL_DEPTH = 160         # ... over up to 4096 rows: 4096 / 256 per team, 4 + 3 in a block, 24 + 5 for partial rows
 
 
 def normed(v, kind, w, b, eps):
