@@ -11,7 +11,9 @@
 // together with the plain entry points of the SpMM / SDDMM families (spmm_host.cu, sddmm_host.cu)
 // and the cache of transposed graphs that their backward passes gather over.  The relational,
 // typed-GEMM and scheduling entry points are bound from Python (cxgnncomp_backend/_typed.py,
-// _rel.py, _schedule.py) on the same C ABI.
+// _rel.py, _schedule.py) on the same C ABI.  Residual norms, rows in 8 bits and the linear map that keeps
+// its input in them (no counterpart in the reference) are here as well: on mini-batches their time is
+// the host's.
 //
 // Differences from the reference's module, all deliberate: errors are Python exceptions
 // (ValueError for bad arguments, RuntimeError otherwise), not exit(1); autograd contexts keep the
@@ -1262,11 +1264,11 @@ struct PackedLinearFunction : public torch::autograd::Function<PackedLinearFunct
     const Tensor &weight = saved[0], g = grads[0];
     const Tensor rows = g.reshape({-1, g.size(-1)});
     tensor_list out(5);
-    if (how[2]) out[0] = at::matmul(g, weight);
+    if (how[2]) out[0] = at::matmul(g, weight.to(g.scalar_type()));      // (autocast: the output is narrower than the weight)
     if (how[3]) {                              // the bias gradient comes out of the same pass over g
       auto [gw, gb] = packed_wgrad(saved[1], saved[2], how[1], how[0], rows, c10::nullopt, c10::nullopt, c10::nullopt, how[4]);
-      out[1] = gw[0].t().to(weight.scalar_type());
-      if (how[4]) out[2] = (*gb)[0].to(g.scalar_type());
+      out[1] = gw[0].t();                      // (autograd rounds both to the parameters' types)
+      if (how[4]) out[2] = (*gb)[0];
     } else if (how[4]) {
       out[2] = rows.sum(0);
     }

@@ -481,11 +481,11 @@ class PackedLinearOP(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             gx = _typed.dense_linear(g, weight) if g.dim() == 2 else None
             if gx is None:
-                gx = g @ weight
+                gx = g @ weight.to(g.dtype)          # (autocast: the output is narrower than the weight)
         if ctx.needs_input_grad[1]:
             packed = PackedRows(codes, exps, ctx.shape[-1], ctx.fmt)
             gw, gb = packed_weight_grad(packed, g.reshape(-1, g.shape[-1]), want_sums=True)
-            gw, gb = gw[0].t().to(weight.dtype), gb[0].to(g.dtype) if ctx.needs_input_grad[2] else None
+            gw, gb = gw[0].t(), gb[0] if ctx.needs_input_grad[2] else None      # (autograd rounds to the parameters' types)
         elif ctx.needs_input_grad[2]:
             gb = g.reshape(-1, g.shape[-1]).sum(dim=0)
         return gx, gw, gb, g if ctx.needs_input_grad[3] else None, None

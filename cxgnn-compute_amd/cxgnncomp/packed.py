@@ -72,7 +72,7 @@ def packed_weight_grad(packed, g, seg_ptr=None, src_idx=None, dst_idx=None, want
     segment of all rows.  The row maps (int64) may be missing: row i.  An entry outside its matrix
     (padding) leaves the row out.  ``want_sums``: returns (gW, gB), gB [R, N] the sums of the same rows of g (the
     bias gradient), from the same pass.  Products are exact up to fp32 accumulation, in a fixed order: results
-    repeat bit for bit."""
+    repeat bit for bit.  Not differentiable."""
     gw, gb = _ops._C.packed_wgrad(packed.codes, packed.exps, packed.cols, FORMATS[packed.fmt], g, seg_ptr, src_idx, dst_idx,
                                   want_sums)
     return (gw, gb) if want_sums else gw

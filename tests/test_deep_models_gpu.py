@@ -122,6 +122,27 @@ def test_linear_in_bf16_and_with_frozen_weights():
 
 
 @gpu
+@pytest.mark.parametrize("m", [300, 5000])
+def test_linear_under_autocast_and_without_rows(m):
+    import cxgnncomp
+    torch.manual_seed(4)
+    x, w, b = (torch.randn(s, device="cuda").requires_grad_(True) for s in ((m, 90), (33, 90), (33, )))
+    announce("linear checkpoint under autocast")
+    with torch.autocast("cuda", dtype=BF16):
+        out = cxgnncomp.linear(x, w, b, checkpoint="int8")
+    assert out.dtype == BF16
+    g = torch.randn(m, 33, device="cuda").to(BF16)
+    gx, gw, gb = torch.autograd.grad(out, (x, w, b), g)
+    assert gx.dtype == gw.dtype == gb.dtype == F32
+    want = packed_ref.weight_grad(packed_ref.pack(x.detach().cpu(), "int8")[2], g.cpu(), [0, m])
+    want.v, want.e = want.v[0].t(), want.e[0].t()
+    check(gw, want, F32, "weight gradient")
+    empty = cxgnncomp.linear(x[:0], w, b, checkpoint="int8")
+    gw, gb = torch.autograd.grad(empty.sum(), (w, b))
+    assert tuple(empty.shape) == (0, 33) and not gw.any() and not gb.any()
+
+
+@gpu
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 def test_typed_linear_that_keeps_its_rows_in_8_bits(fmt):
     import cxgnncomp
