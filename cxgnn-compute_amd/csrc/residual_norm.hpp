@@ -27,53 +27,75 @@ struct RnArgs {
   float* partial;                        // [blocks][kRnSums][cols]
 };
 
-// How the last piece of a row ends: with the row; short, its values then come from the V last columns; or
-// the whole row is shorter than one piece.
+// How the last piece of a row ends: with the row; past it, the piece is then moved back to end with the
+// row; or the whole row is shorter than one piece.
 enum RnTail { kRnWhole, kRnShort, kRnTiny };
 
 // A team of L lanes owns a row, PER columns per lane; narrow rows share a wave, wide ones take several
 // waves.  Piece i of lane l starts at column (i * L + l) * V: each load of a team is one contiguous run.
+// A piece that was moved back holds columns that its neighbour holds too: both compute and store the same
+// values for them, and sums over a row leave the second one's out.
 template <typename TX, typename TF, int L_, int PER_, int TAIL_> struct RnTeam {
   static constexpr int L = L_, PER = PER_, V = 16 / (sizeof(TX) > sizeof(TF) ? sizeof(TX) : sizeof(TF)), ITEMS = PER / V;
   static constexpr int THREADS = L < 256 ? 256 : L, TEAMS = THREADS / L, WAVES = THREADS / CXG_WAVE;
   static constexpr int TAIL = TAIL_;
 };
 
-// V values of a row from column c on, any alignment of the row; zeros where c is past its end.  A short
-// piece is read where it ends with the row, without a branch, and moved to its place by rn_widen.
-template <int TAIL, typename T, int V> __device__ __forceinline__ void rn_load(RowPiece<T, V>& p, const T* row, int c, int cols) {
-  if constexpr (TAIL == kRnTiny) {
-    p.load(row, c, cols);
-  } else {
-    p.t = (T)0.f;
-    if (c < cols) p.t = *reinterpret_cast<const typename RowPiece<T, V>::loose_t*>(row + (TAIL == kRnShort && c + V > cols ? cols - V : c));
-  }
-}
-template <int TAIL, typename T, int V> __device__ __forceinline__ void rn_widen(const RowPiece<T, V>& p, int c, int cols, float (&v)[V]) {
-  p.widen(v);
-  if constexpr (TAIL == kRnShort) {
-    if (c < cols && c + V > cols) {
-      const int s = c + V - cols;                        // 1 .. V - 1 values in front of the piece
+// The pieces of a lane.
+template <typename S> struct RnPieces {
+  int col[S::ITEMS], shared[S::ITEMS];                   // first column; leading values that the neighbour holds
+  bool on[S::ITEMS];
+  int cols;
+  __device__ __forceinline__ RnPieces(int cols_) : cols(cols_) {
+    const int lit = threadIdx.x % S::L;
 #pragma unroll
-      for (int k = V / 2; k >= 1; k /= 2)
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = (s & k) ? (j + k < V ? v[j + k] : 0.f) : v[j];
+    for (int i = 0; i < S::ITEMS; ++i) {
+      const int c = (i * S::L + lit) * S::V;
+      on[i] = c < cols;
+      shared[i] = S::TAIL == kRnShort && on[i] && c + S::V > cols ? c + S::V - cols : 0;
+      col[i] = c - shared[i];
     }
   }
-}
-template <int TAIL, typename T, int V> __device__ __forceinline__ void rn_store(const float (&v)[V], T* row, int c, int cols) {
-  RowPiece<T, V> p;
-  p.narrow(v);
-  if constexpr (TAIL != kRnWhole) {
-    p.store(row, c, cols);
-  } else {
-    if (c < cols) *reinterpret_cast<typename RowPiece<T, V>::loose_t*>(row + c) = p.t;
+  // whether value j of piece i counts in sums over the row
+  __device__ __forceinline__ bool counts(int i, int j) const {
+    return on[i] && (S::TAIL == kRnWhole || (S::TAIL == kRnShort ? j >= shared[i] : col[i] + j < cols));
   }
-}
-
-template <int L, int V> __device__ __forceinline__ int rn_col(int item, int lane_in_team) {
-  return (item * L + lane_in_team) * V;
-}
+  // any alignment of the row; zeros where there is no column
+  template <typename T> __device__ __forceinline__ void load(RowPiece<T, S::V>& p, const T* row, int i, bool live = true) const {
+    p.t = (T)0.f;
+    if constexpr (S::TAIL == kRnTiny) {
+      if (live) p.load(row, col[i], cols);
+    } else {
+      if (on[i] && live) p.t = *reinterpret_cast<const typename RowPiece<T, S::V>::loose_t*>(row + col[i]);
+    }
+  }
+  template <typename T> __device__ __forceinline__ void store(const float (&v)[S::V], T* row, int i) const {
+    RowPiece<T, S::V> p;
+    p.narrow(v);
+    if constexpr (S::TAIL == kRnTiny) {
+      p.store(row, col[i], cols);
+    } else {
+      if (on[i]) *reinterpret_cast<typename RowPiece<T, S::V>::loose_t*>(row + col[i]) = p.t;
+    }
+  }
+  // fp32 parameter vectors: 0 where there is no column, `missing` where there is no vector
+  __device__ __forceinline__ void params(const float* p, float missing, float (&out)[S::ITEMS][S::V]) const {
+#pragma unroll
+    for (int i = 0; i < S::ITEMS; ++i)
+#pragma unroll
+      for (int q = 0; q < S::V; q += 4) {
+        RowPiece<float, 4> w;
+        if (p) {
+          w.load(p, col[i] + q, cols);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w.t[j] = col[i] + q + j < cols ? missing : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) out[i][q + j] = w.t[j];
+      }
+  }
+};
 
 // Sum over the team; every lane gets it.  Teams of several waves meet in LDS (`slot` alternates between
 // two buffers, so that one barrier per sum is enough).
@@ -98,26 +120,6 @@ __device__ __forceinline__ void team_sum(float (&v)[N], float (*s_red)[S::WAVES]
     }
     slot ^= 1;
   }
-}
-
-// fp32 parameter vectors: 0 where there is no column, `missing` where there is no vector
-template <int L, int V, int ITEMS>
-__device__ __forceinline__ void rn_params(const float* p, int cols, int lit, float missing, float (&out)[ITEMS][V]) {
-#pragma unroll
-  for (int i = 0; i < ITEMS; ++i)
-#pragma unroll
-    for (int q = 0; q < V; q += 4) {
-      const int c = rn_col<L, V>(i, lit) + q;
-      RowPiece<float, 4> w;
-      if (p) {
-        w.load(p, c, cols);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w.t[j] = c + j < cols ? missing : 0.f;
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) out[i][q + j] = w.t[j];
-    }
 }
 
 // F<TX, TF, L, PER, TAIL>(a, st) for the types and the width: 8 columns per lane (16 are no faster where

@@ -31,16 +31,16 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_bwd_kernel(RnArgs a)
   const int lit = threadIdx.x % L, team = threadIdx.x / L;
   const int cols = a.cols;
   const float inv_c = 1.0f / (float)cols;
+  const RnPieces<S> at(cols);
   int slot = 0;
   const bool post = a.post_kind != CXG_NORM_NONE, pre = a.pre_kind != CXG_NORM_NONE;
   const bool post_layer = a.post_kind == CXG_NORM_LAYER, pre_layer = a.pre_kind == CXG_NORM_LAYER;
   float w1[ITEMS][V], b1[ITEMS][V], w2[ITEMS][V], gc[ITEMS][V];
   // columns that do not exist have weight 0 and so add nothing to the sums over a row
-  rn_params<L, V, ITEMS>(post ? a.post_w : nullptr, cols, lit, 1.f, w1);
-  rn_params<L, V, ITEMS>(post ? a.post_b : nullptr, cols, lit, 0.f, b1);
-  rn_params<L, V, ITEMS>(pre ? a.pre_w : nullptr, cols, lit, 1.f, w2);
-  rn_params<L, V, ITEMS>(a.gate_kind == CXG_GATE_CHANNEL ? static_cast<const float*>(a.gate) : nullptr, cols, lit, 1.f, gc);
-  auto inside = [&](int i, int j) { return rn_col<L, V>(i, lit) + (S::TAIL != kRnWhole ? j : 0) < cols; };
+  at.params(post ? a.post_w : nullptr, 1.f, w1);
+  at.params(post ? a.post_b : nullptr, 0.f, b1);
+  at.params(pre ? a.pre_w : nullptr, 1.f, w2);
+  at.params(a.gate_kind == CXG_GATE_CHANNEL ? static_cast<const float*>(a.gate) : nullptr, 1.f, gc);
   float sums[kRnSums][ITEMS][V];
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i)
@@ -56,17 +56,15 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_bwd_kernel(RnArgs a)
     RowPiece<TX, V> px[ITEMS], pdr[ITEMS];
     RowPiece<TF, V> pf[ITEMS], pg[ITEMS], pdy[ITEMS];
     const bool full = a.gate_kind == CXG_GATE_FULL;
-    const int here = live ? cols : 0;                     // a row that does not exist adds zeros everywhere
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      const int c = rn_col<L, V>(i, lit);
-      px[i].t = pdr[i].t = (TX)0.f;
+    for (int i = 0; i < ITEMS; ++i) {                     // a row that does not exist adds zeros everywhere
       pf[i].t = pg[i].t = pdy[i].t = (TF)0.f;
-      rn_load<S::TAIL>(px[i], static_cast<const TX*>(a.x) + rr * a.ldx, c, here);
-      if (a.f) rn_load<S::TAIL>(pf[i], static_cast<const TF*>(a.f) + rr * a.ldf, c, here);
-      if (a.dr) rn_load<S::TAIL>(pdr[i], static_cast<const TX*>(a.dr) + rr * a.lddr, c, here);
-      if (a.dy) rn_load<S::TAIL>(pdy[i], static_cast<const TF*>(a.dy) + rr * a.lddy, c, here);
-      if (full) rn_load<S::TAIL>(pg[i], static_cast<const TF*>(a.gate) + rr * a.ldg, c, here);
+      pdr[i].t = (TX)0.f;
+      at.load(px[i], static_cast<const TX*>(a.x) + rr * a.ldx, i, live);
+      if (a.f) at.load(pf[i], static_cast<const TF*>(a.f) + rr * a.ldf, i, live);
+      if (a.dr) at.load(pdr[i], static_cast<const TX*>(a.dr) + rr * a.lddr, i, live);
+      if (a.dy) at.load(pdy[i], static_cast<const TF*>(a.dy) + rr * a.lddy, i, live);
+      if (full) at.load(pg[i], static_cast<const TF*>(a.gate) + rr * a.ldg, i, live);
     }
     const float grow = a.gate_kind == CXG_GATE_ROW && live ? (float)static_cast<const TF*>(a.gate)[rr * a.ldg] : 1.f;
     float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
@@ -77,12 +75,11 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_bwd_kernel(RnArgs a)
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       float x[V], f[V], dy[V], gf[V];
-      const int c = rn_col<L, V>(i, lit);
-      rn_widen<S::TAIL>(px[i], c, cols, x);
-      rn_widen<S::TAIL>(pf[i], c, cols, f);
-      rn_widen<S::TAIL>(pdy[i], c, cols, dy);
-      rn_widen<S::TAIL>(pg[i], c, cols, gf);
-      rn_widen<S::TAIL>(pdr[i], c, cols, g[i]);
+      px[i].widen(x);
+      pf[i].widen(f);
+      pdy[i].widen(dy);
+      pg[i].widen(gf);
+      pdr[i].widen(g[i]);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         fh[i][j] = post ? (f[j] - st.x) * st.y : f[j];
@@ -92,8 +89,9 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_bwd_kernel(RnArgs a)
         const float r = a.res_scale * x[j] + a.branch_scale * grow * hg;
         rh[i][j] = (r - st.z) * st.w;
         const float t = dy[j] * w2[i][j];
-        s[0] += t;
-        s[1] += t * rh[i][j];
+        const float tc = S::TAIL != kRnShort || at.counts(i, j) ? t : 0.f;
+        s[0] += tc;
+        s[1] += tc * rh[i][j];
         sums[0][i][j] += dy[j] * rh[i][j];
         sums[1][i][j] += dy[j];
       }
@@ -104,7 +102,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_bwd_kernel(RnArgs a)
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
         float dy[V];
-        rn_widen<S::TAIL>(pdy[i], rn_col<L, V>(i, lit), cols, dy);
+        pdy[i].widen(dy);
 #pragma unroll
         for (int j = 0; j < V; ++j) g[i][j] += st.w * (dy[j] * w2[i][j] - m0 - rh[i][j] * m1);
       }
@@ -116,7 +114,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_bwd_kernel(RnArgs a)
         float o[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) o[j] = a.res_scale * g[i][j];
-        rn_store<S::TAIL>(o, out, rn_col<L, V>(i, lit), cols);
+        at.store(o, out, i);
       }
     }
     if (a.dgate) {
@@ -128,7 +126,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_bwd_kernel(RnArgs a)
             float o[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) o[j] = a.branch_scale * g[i][j] * h[i][j];
-            rn_store<S::TAIL>(o, out, rn_col<L, V>(i, lit), cols);
+            at.store(o, out, i);
           }
         }
       } else if (a.gate_kind == CXG_GATE_ROW) {
@@ -136,7 +134,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_bwd_kernel(RnArgs a)
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-          for (int j = 0; j < V; ++j) d[0] += inside(i, j) ? g[i][j] * h[i][j] : 0.f;
+          for (int j = 0; j < V; ++j) d[0] += at.counts(i, j) ? g[i][j] * h[i][j] : 0.f;
         team_sum<S, 1>(d, s_red, slot);
         if (live && lit == 0) static_cast<TF*>(a.dgate)[rr] = (TF)(a.branch_scale * d[0]);
       }
@@ -151,8 +149,9 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_bwd_kernel(RnArgs a)
           sums[2][i][j] += cg * fh[i][j];
           sums[3][i][j] += cg;
           g[i][j] = a.branch_scale * cg * (full ? 1.f : gc[i][j]) * w1[i][j];
-          q[0] += g[i][j];
-          q[1] += g[i][j] * fh[i][j];
+          const float gc_ = S::TAIL != kRnShort || at.counts(i, j) ? g[i][j] : 0.f;
+          q[0] += gc_;
+          q[1] += gc_ * fh[i][j];
         }
       if (a.df) {
         float m0 = 0.f, m1 = 0.f;
@@ -168,7 +167,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_bwd_kernel(RnArgs a)
             float o[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) o[j] = post ? st.y * (g[i][j] - m0 - fh[i][j] * m1) : g[i][j];
-            rn_store<S::TAIL>(o, out, rn_col<L, V>(i, lit), cols);
+            at.store(o, out, i);
           }
         }
       }
@@ -185,7 +184,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_bwd_kernel(RnArgs a)
       for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const int c = rn_col<L, V>(i, lit) + j;
+          const int c = at.col[i] + j;
           if (c < cols) out[(size_t)q * cols + c] = sums[q][i][j];
         }
   } else {
@@ -200,7 +199,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_bwd_kernel(RnArgs a)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const float t = groups_sum<L>(sums[q][i][j]);
-          if (L >= CXG_WAVE || (int)(threadIdx.x & (CXG_WAVE - 1)) < L) s_col[part][rn_col<L, V>(i, lit) + j] = t;
+          if (L >= CXG_WAVE || (int)(threadIdx.x & (CXG_WAVE - 1)) < L) s_col[part][at.col[i] + j] = t;
         }
       __syncthreads();
       for (int c = threadIdx.x; c < cols; c += S::THREADS) {

@@ -51,18 +51,18 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a)
   const int lit = threadIdx.x % L, team = threadIdx.x / L;
   const int cols = a.cols;
   const float inv_c = 1.0f / (float)cols;
+  const RnPieces<S> at(cols);
   int slot = 0;
   float w1[ITEMS][V], b1[ITEMS][V], w2[ITEMS][V], b2[ITEMS][V], gc[ITEMS][V];
   if (a.post_kind != CXG_NORM_NONE) {
-    rn_params<L, V, ITEMS>(a.post_w, cols, lit, 1.f, w1);
-    rn_params<L, V, ITEMS>(a.post_b, cols, lit, 0.f, b1);
+    at.params(a.post_w, 1.f, w1);
+    at.params(a.post_b, 0.f, b1);
   }
   if (a.pre_kind != CXG_NORM_NONE) {
-    rn_params<L, V, ITEMS>(a.pre_w, cols, lit, 1.f, w2);
-    rn_params<L, V, ITEMS>(a.pre_b, cols, lit, 0.f, b2);
+    at.params(a.pre_w, 1.f, w2);
+    at.params(a.pre_b, 0.f, b2);
   }
-  if (a.gate_kind == CXG_GATE_CHANNEL) rn_params<L, V, ITEMS>(static_cast<const float*>(a.gate), cols, lit, 1.f, gc);
-  auto inside = [&](int i, int j) { return rn_col<L, V>(i, lit) + (S::TAIL != kRnWhole ? j : 0) < cols; };
+  if (a.gate_kind == CXG_GATE_CHANNEL) at.params(static_cast<const float*>(a.gate), 1.f, gc);
 
   // every lane stays in the loop as long as its block: the reductions need whole waves
   for (int64_t base = (int64_t)blockIdx.x * kTeams; base < a.rows; base += (int64_t)gridDim.x * kTeams) {
@@ -73,17 +73,17 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a)
     RowPiece<TF, V> pf[ITEMS], pg[ITEMS];
     const TX* const xrow = static_cast<const TX*>(a.x) + rr * a.ldx;
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) rn_load<S::TAIL>(px[i], xrow, rn_col<L, V>(i, lit), cols);
+    for (int i = 0; i < ITEMS; ++i) at.load(px[i], xrow, i);
     if (a.f) {
       const TF* const frow = static_cast<const TF*>(a.f) + rr * a.ldf;
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i) rn_load<S::TAIL>(pf[i], frow, rn_col<L, V>(i, lit), cols);
+      for (int i = 0; i < ITEMS; ++i) at.load(pf[i], frow, i);
     }
     float grow = 1.f;
     if (a.gate_kind == CXG_GATE_FULL) {
       const TF* const gr = static_cast<const TF*>(a.gate) + rr * a.ldg;
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i) rn_load<S::TAIL>(pg[i], gr, rn_col<L, V>(i, lit), cols);
+      for (int i = 0; i < ITEMS; ++i) at.load(pg[i], gr, i);
     } else if (a.gate_kind == CXG_GATE_ROW) {
       grow = (float)static_cast<const TF*>(a.gate)[rr * a.ldg];
     }
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a)
     float mean1 = 0.f, rstd1 = 1.f, mean2 = 0.f, rstd2 = 1.f;
     if (a.f) {
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i) rn_widen<S::TAIL>(pf[i], rn_col<L, V>(i, lit), cols, v[i]);
+      for (int i = 0; i < ITEMS; ++i) pf[i].widen(v[i]);
       if (a.post_kind != CXG_NORM_NONE) {
         float s[1];
         if (a.post_kind == CXG_NORM_LAYER) {
@@ -100,7 +100,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a)
 #pragma unroll
           for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-            for (int j = 0; j < V; ++j) s[0] += v[i][j];
+            for (int j = 0; j < V; ++j) s[0] += S::TAIL != kRnShort || at.counts(i, j) ? v[i][j] : 0.f;
           team_sum<S, 1>(s, s_red, slot);
           mean1 = s[0] * inv_c;
         }
@@ -109,8 +109,8 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a)
         for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            v[i][j] = inside(i, j) ? v[i][j] - mean1 : 0.f;
-            s[0] += v[i][j] * v[i][j];
+            v[i][j] -= mean1;
+            s[0] += at.counts(i, j) ? v[i][j] * v[i][j] : 0.f;
           }
         team_sum<S, 1>(s, s_red, slot);
         rstd1 = 1.0f / sqrtf(s[0] * inv_c + a.eps);
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a)
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
           float g[V];
-          rn_widen<S::TAIL>(pg[i], rn_col<L, V>(i, lit), cols, g);
+          pg[i].widen(g);
 #pragma unroll
           for (int j = 0; j < V; ++j) v[i][j] *= g[j];
         }
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a)
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
         float x[V];
-        rn_widen<S::TAIL>(px[i], rn_col<L, V>(i, lit), cols, x);
+        px[i].widen(x);
 #pragma unroll
         for (int j = 0; j < V; ++j) v[i][j] = a.res_scale * x[j] + bs * v[i][j];
       }
@@ -145,7 +145,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a)
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
         float x[V];
-        rn_widen<S::TAIL>(px[i], rn_col<L, V>(i, lit), cols, x);
+        px[i].widen(x);
 #pragma unroll
         for (int j = 0; j < V; ++j) v[i][j] = a.res_scale * x[j];
       }
@@ -153,7 +153,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a)
     if (a.r && live) {
       TX* const out = static_cast<TX*>(a.r) + rr * cols;
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i) rn_store<S::TAIL>(v[i], out, rn_col<L, V>(i, lit), cols);
+      for (int i = 0; i < ITEMS; ++i) at.store(v[i], out, i);
     }
     if (a.pre_kind != CXG_NORM_NONE) {
       float s[1];
@@ -162,7 +162,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a)
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-          for (int j = 0; j < V; ++j) s[0] += v[i][j];
+          for (int j = 0; j < V; ++j) s[0] += S::TAIL != kRnShort || at.counts(i, j) ? v[i][j] : 0.f;
         team_sum<S, 1>(s, s_red, slot);
         mean2 = s[0] * inv_c;
       }
@@ -171,8 +171,8 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a)
       for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          v[i][j] = inside(i, j) ? v[i][j] - mean2 : 0.f;
-          s[0] += v[i][j] * v[i][j];
+          v[i][j] -= mean2;
+          s[0] += at.counts(i, j) ? v[i][j] * v[i][j] : 0.f;
         }
       team_sum<S, 1>(s, s_red, slot);
       rstd2 = 1.0f / sqrtf(s[0] * inv_c + a.eps);
@@ -183,7 +183,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a)
           float o[V];
 #pragma unroll
           for (int j = 0; j < V; ++j) o[j] = v[i][j] * rstd2 * w2[i][j] + b2[i][j];
-          rn_store<S::TAIL>(o, out, rn_col<L, V>(i, lit), cols);
+          at.store(o, out, i);
         }
       }
     }
