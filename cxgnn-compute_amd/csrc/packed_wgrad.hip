@@ -421,8 +421,7 @@ int64_t pw_chunk_rows(int64_t M, int K, int N, int R) {
   const int64_t longest = fill(1), shortest = fill(2);
   int64_t rows = 2048;
   rows = rows > longest ? longest : rows < shortest ? shortest : rows;
-  rows = ceil_div(rows, (int64_t)64) * 64;
-  return rows < 128 ? 128 : rows;
+  return rows < 1 ? 64 : ceil_div(rows, (int64_t)64) * 64;
 }
 
 int64_t pw_chunk_count(int64_t M, int K, int N, int R) {
