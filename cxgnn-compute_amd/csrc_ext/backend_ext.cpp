@@ -990,7 +990,7 @@ struct ResidualNorm {
   const float* vec(int i) const { return t[i].defined() ? (const float*)t[i].data_ptr() : nullptr; }
   const void* ptr(int i) const { return t[i].defined() ? t[i].data_ptr() : nullptr; }
   int64_t ld(int i) const { return t[i].defined() && t[i].dim() == 2 ? t[i].stride(0) : 0; }
-  Tensor matrix(at::ScalarType dtype) const { return torch::empty({rows, cols}, t[kRnX].options().dtype(dtype).requires_grad(false)); }
+  Tensor matrix(at::ScalarType dtype) const { return at::empty({rows, cols}, t[kRnX].options().dtype(dtype).requires_grad(false)); }
 };
 
 void rn_vector(Tensor& v, const char* name, const ResidualNorm& c) {
@@ -1044,7 +1044,7 @@ void rn_prepare(ResidualNorm& c) {
 void rn_forward(const ResidualNorm& c, Tensor& r, Tensor& y, Tensor* stats) {
   if (c.t[kRnF].defined()) r = c.matrix(c.t[kRnX].scalar_type());
   if (c.pre != CXG_NORM_NONE) y = c.matrix(c.branch_dtype);
-  if (stats) *stats = torch::empty({c.rows, 4}, c.t[kRnX].options().dtype(at::kFloat).requires_grad(false));
+  if (stats) *stats = at::empty({c.rows, 4}, c.t[kRnX].options().dtype(at::kFloat).requires_grad(false));
   c10::DeviceGuard guard(c.t[kRnX].device());
   check(cxg_residual_norm_fwd(c.ptr(kRnX), c.ld(kRnX), c.ptr(kRnF), c.ld(kRnF), c.ptr(kRnGate), c.ld(kRnGate), c.gate_kind, c.post,
                               c.vec(kRnPostW), c.vec(kRnPostB), c.pre, c.vec(kRnPreW), c.vec(kRnPreB), (float)c.res_scale,
@@ -1103,12 +1103,12 @@ struct ResidualNormFunction : public torch::autograd::Function<ResidualNormFunct
     if (need[kRnX]) out[kRnX] = c.matrix(c.t[kRnX].scalar_type());
     if (need[kRnF]) out[kRnF] = c.matrix(c.branch_dtype);
     if (need[kRnGate])
-      out[kRnGate] = c.gate_kind == CXG_GATE_CHANNEL ? torch::empty({c.cols}, fp32)
-                                                     : torch::empty(c.t[kRnGate].sizes(), fp32.dtype(c.branch_dtype));
+      out[kRnGate] = c.gate_kind == CXG_GATE_CHANNEL ? at::empty({c.cols}, fp32)
+                                                     : at::empty(c.t[kRnGate].sizes(), fp32.dtype(c.branch_dtype));
     bool sums = need[kRnGate] && c.gate_kind == CXG_GATE_CHANNEL;
     for (int i = kRnPostW; i < kRnTensors; ++i)
       if (need[i]) {
-        out[i] = torch::empty({c.cols}, fp32);
+        out[i] = at::empty({c.cols}, fp32);
         sums = true;
       }
     Tensor ws;
@@ -1173,8 +1173,8 @@ std::tuple<Tensor, Tensor> pack_rows(const Tensor& x_in, int64_t fmt) {
   const int64_t rows = x.size(0), cols = x.size(1);
   if (cols < 1 || cols > INT32_MAX) bad(fmt_cols(cols));
   const auto bytes = x.options().dtype(at::kByte).requires_grad(false);
-  Tensor codes = torch::empty({rows, (int64_t)cxg_packed_pitch((int)cols)}, bytes);
-  Tensor exps = torch::empty({rows, (int64_t)cxg_packed_groups((int)cols)}, bytes);
+  Tensor codes = at::empty({rows, (int64_t)cxg_packed_pitch((int)cols)}, bytes);
+  Tensor exps = at::empty({rows, (int64_t)cxg_packed_groups((int)cols)}, bytes);
   c10::DeviceGuard guard(x.device());
   check(cxg_pack_rows(ptr_or_null(x), x.stride(0), value_type(x, "x"), (int)fmt, rows, (int)cols, (uint8_t*)ptr_or_null_mut(codes),
                       (uint8_t*)ptr_or_null_mut(exps), stream_of(x)));
@@ -1194,7 +1194,7 @@ void req_packed(const Tensor& codes, const Tensor& exps, int64_t cols) {
 
 Tensor unpack_rows(const Tensor& codes, const Tensor& exps, int64_t cols, int64_t fmt, const py::object& dtype) {
   req_packed(codes, exps, cols);
-  Tensor out = torch::empty({codes.size(0), cols}, codes.options().dtype(torch::python::detail::py_object_to_dtype(dtype)));
+  Tensor out = at::empty({codes.size(0), cols}, codes.options().dtype(torch::python::detail::py_object_to_dtype(dtype)));
   c10::DeviceGuard guard(codes.device());
   check(cxg_unpack_rows((const uint8_t*)ptr_or_null(codes), (const uint8_t*)ptr_or_null(exps), (int)fmt, codes.size(0), (int)cols,
                         ptr_or_null_mut(out), value_type(out, "the unpacked rows"), stream_of(codes)));
@@ -1228,9 +1228,9 @@ std::tuple<Tensor, OptTensor> packed_wgrad(const Tensor& codes, const Tensor& ex
     segs = seg->size(0) - 1;
     if (segs < 1) bad("seg_ptr needs at least two entries");
   }
-  Tensor gw = torch::empty({segs, cols, g.size(1)}, codes.options().dtype(at::kFloat));
+  Tensor gw = at::empty({segs, cols, g.size(1)}, codes.options().dtype(at::kFloat));
   OptTensor gb;
-  if (want_sums) gb = torch::empty({segs, g.size(1)}, gw.options());
+  if (want_sums) gb = at::empty({segs, g.size(1)}, gw.options());
   const int K = (int)cols, N = (int)g.size(1), R = (int)segs;
   Tensor ws = workspace(cxg_packed_wgrad_workspace_bytes(rows, K, N, R), codes);
   c10::DeviceGuard guard(codes.device());
