@@ -74,9 +74,13 @@ class TypedLinearE2EOP(torch.autograd.Function):
         sorted_types = new_types[indices]
         return [sorted_types, num_item, indices, count.cpu()]
 
+    @classmethod
+    def apply(cls, x, weights, types, preprocessed=[], thres=256, count=None, checkpoint=None):
+        check_format(checkpoint)
+        return super().apply(x, weights, types, preprocessed, thres, count, checkpoint if torch.is_grad_enabled() else None)
+
     @staticmethod
     def forward(ctx, x, weights, types, preprocessed=[], thres=256, count=None, checkpoint=None):
-        check_format(checkpoint)
         if len(preprocessed) == 4:
             sorted_types, num_item, indices, count = preprocessed
         else:

@@ -122,6 +122,39 @@ def test_linear_in_bf16_and_with_frozen_weights():
 
 
 @gpu
+def test_nothing_is_packed_where_no_backward_pass_follows(monkeypatch):
+    """Without gradients (serving) a layer's input is not packed; bad formats are refused all the same."""
+    import cxgnncomp
+    from cxgnncomp import graph_conv, typed_linear
+    from cxgnncomp_backend import _ops
+
+    class NoPacking:
+        def __getattr__(self, name):
+            assert name not in ("pack_rows", "packed_linear")
+            return getattr(_native, name)
+
+    def no_packing(*a):
+        raise AssertionError("packed")
+
+    _native = _ops._C
+    monkeypatch.setattr(graph_conv, "pack_rows", no_packing)
+    monkeypatch.setattr(typed_linear, "pack_rows", no_packing)
+    monkeypatch.setattr(_ops, "_C", NoPacking())
+    x, w = torch.randn(5000, 64, device="cuda"), torch.randn(32, 64, device="cuda", requires_grad=True)
+    w3, types = torch.randn(3, 64, 32, device="cuda", requires_grad=True), torch.randint(0, 3, (5000, ), device="cuda")
+    announce("linear checkpoint without gradients")
+    with torch.no_grad():
+        assert torch.equal(cxgnncomp.linear(x, w, checkpoint="int8"), cxgnncomp.linear(x, w))
+        assert torch.equal(cxgnncomp.linear(x[:9], w, checkpoint="int8"), cxgnncomp.linear(x[:9], w))
+        a = cxgnncomp.TypedLinearE2EOP.apply(x, w3, types, [], 256, None, "int8")
+        assert torch.equal(a, cxgnncomp.TypedLinearE2EOP.apply(x, w3, types))
+        with pytest.raises(ValueError):
+            cxgnncomp.TypedLinearE2EOP.apply(x, w3, types, [], 256, None, "int4")
+    with pytest.raises(AssertionError):
+        cxgnncomp.linear(x, w, checkpoint="int8")
+
+
+@gpu
 @pytest.mark.parametrize("m", [300, 5000])
 def test_linear_under_autocast_and_without_rows(m):
     import cxgnncomp
