@@ -14,8 +14,8 @@
 // Layout: codes [rows][pitch] with the columns rounded up to 16 (zeros behind the last), one
 // exponent byte k + 127 per group, [rows][groups].
 //
-// Bound: memory, one pass.  Eight lanes own a group and hold its 128 values in registers between the
-// maximum (integer maxima of the magnitudes' bits, so that a NaN is largest; three data-parallel
+// Bound: memory, one pass.  Eight lanes own a group (two where a row is that short) and hold its values in registers between
+// the maximum (integer maxima of the magnitudes' bits, so that a NaN is largest; three data-parallel
 // moves) and the rounding; a piece of the group is 128 contiguous bytes over the eight lanes.
 // Measured: 2,449,029 x 128 fp32 packed in 289 us = 5.4 TB/s (a 4 GiB copy: 4.7 TB/s).
 #include "packed_rows.hpp"
@@ -24,8 +24,10 @@ namespace cxg {
 namespace {
 
 constexpr int kPrThreads = 256;
-constexpr int kPrLanes = 8;                              // lanes per group
-constexpr int kPrTeams = kPrThreads / kPrLanes;          // rows per block step
+// Lanes per group, sixteen columns each: eight, or two for rows of at most 32 columns (48 M bf16 values in
+// rows of 16: 28 us against 82 us).
+constexpr int kPrLanes = 8, kPrLanesNarrow = 2;
+inline bool pr_narrow(int cols) { return cols <= 16 * kPrLanesNarrow; }
 
 struct PackArgs {
   const void* x; int64_t ldx;
@@ -65,18 +67,18 @@ template <int FMT> __device__ __forceinline__ unsigned encode4(const float* v, f
   }
 }
 
-template <typename T, int FMT> __global__ __launch_bounds__(kPrThreads) void pack_rows_kernel(PackArgs a) {
-  constexpr int V = 16 / sizeof(T), kPieces = kPrGroup / (kPrLanes * V);
-  const int lit = threadIdx.x % kPrLanes, group = blockIdx.y;
+template <typename T, int FMT, int LANES> __global__ __launch_bounds__(kPrThreads) void pack_rows_kernel(PackArgs a) {
+  constexpr int V = 16 / sizeof(T), kPieces = 16 / V, kTeams = kPrThreads / LANES;
+  const int lit = threadIdx.x % LANES, group = blockIdx.y;
   const int c0 = group * kPrGroup;
-  for (int64_t base = (int64_t)blockIdx.x * kPrTeams; base < a.rows; base += (int64_t)gridDim.x * kPrTeams) {
-    const int64_t row = base + threadIdx.x / kPrLanes;
+  for (int64_t base = (int64_t)blockIdx.x * kTeams; base < a.rows; base += (int64_t)gridDim.x * kTeams) {
+    const int64_t row = base + threadIdx.x / LANES;
     const bool live = row < a.rows;                      // dead teams stay: the moves need whole waves
     const T* const src = static_cast<const T*>(a.x) + (live ? row : 0) * a.ldx;
     float v[kPieces][V];
     RowPiece<T, V> raw[kPieces];
 #pragma unroll
-    for (int p = 0; p < kPieces; ++p) raw[p].load(src, c0 + (p * kPrLanes + lit) * V, a.cols);
+    for (int p = 0; p < kPieces; ++p) raw[p].load(src, c0 + (p * LANES + lit) * V, a.cols);
     unsigned top = 0;
 #pragma unroll
     for (int p = 0; p < kPieces; ++p) {
@@ -88,14 +90,16 @@ template <typename T, int FMT> __global__ __launch_bounds__(kPrThreads) void pac
       }
     }
     top = moved_max<0xB1>(top);                          // quad_perm [1,0,3,2]
-    top = moved_max<0x4E>(top);                          // quad_perm [2,3,0,1]
-    top = moved_max<0x141>(top);                         // row_half_mirror
+    if constexpr (LANES == 8) {
+      top = moved_max<0x4E>(top);                        // quad_perm [2,3,0,1]
+      top = moved_max<0x141>(top);                       // row_half_mirror
+    }
     const int b = exponent_byte<FMT>(top);
     const float inv = __uint_as_float((unsigned)(254 - b) << 23);
     if (!live) continue;
 #pragma unroll
     for (int p = 0; p < kPieces; ++p) {
-      const int c = c0 + (p * kPrLanes + lit) * V;
+      const int c = c0 + (p * LANES + lit) * V;
       if (c >= a.pitch) continue;
       uint8_t* const dst = a.codes + row * a.pitch + c;
       unsigned w[V / 4];
@@ -111,17 +115,17 @@ template <typename T, int FMT> __global__ __launch_bounds__(kPrThreads) void pac
   }
 }
 
-template <typename T, int FMT> __global__ __launch_bounds__(kPrThreads) void unpack_rows_kernel(PackArgs a) {
-  constexpr int V = 16 / sizeof(T), kPieces = kPrGroup / (kPrLanes * V);
-  const int lit = threadIdx.x % kPrLanes, group = blockIdx.y;
+template <typename T, int FMT, int LANES> __global__ __launch_bounds__(kPrThreads) void unpack_rows_kernel(PackArgs a) {
+  constexpr int V = 16 / sizeof(T), kPieces = 16 / V, kTeams = kPrThreads / LANES;
+  const int lit = threadIdx.x % LANES, group = blockIdx.y;
   const int c0 = group * kPrGroup;
-  for (int64_t row = (int64_t)blockIdx.x * kPrTeams + threadIdx.x / kPrLanes; row < a.rows;
-       row += (int64_t)gridDim.x * kPrTeams) {
+  for (int64_t row = (int64_t)blockIdx.x * kTeams + threadIdx.x / LANES; row < a.rows;
+       row += (int64_t)gridDim.x * kTeams) {
     const uint8_t* const src = a.codes + row * a.pitch;
     unsigned w[kPieces][V / 4];
 #pragma unroll
     for (int p = 0; p < kPieces; ++p) {
-      const int c = c0 + (p * kPrLanes + lit) * V;
+      const int c = c0 + (p * LANES + lit) * V;
 #pragma unroll
       for (int q = 0; q < V / 4; ++q) w[p][q] = 0;
       if (c < a.pitch) {
@@ -142,7 +146,7 @@ template <typename T, int FMT> __global__ __launch_bounds__(kPrThreads) void unp
       for (int q = 0; q < V / 4; ++q) decode4<FMT>(w[p][q], scale, &v[4 * q]);
       RowPiece<T, V> o;
       o.narrow(v);
-      o.store(dst, c0 + (p * kPrLanes + lit) * V, a.cols);
+      o.store(dst, c0 + (p * LANES + lit) * V, a.cols);
     }
   }
 }
@@ -155,26 +159,31 @@ int pack_check(int type, int fmt, int64_t rows, int cols) {
   return CXG_OK;
 }
 
-dim3 pack_grid(int64_t rows, int groups) {
-  int64_t x = ceil_div(rows, (int64_t)kPrTeams);
+dim3 pack_grid(int64_t rows, int groups, int teams) {
+  int64_t x = ceil_div(rows, (int64_t)teams);
   const int64_t most = groups >= 64 ? 256 : 16384 / groups;      // rows per block beyond that: a loop
   return dim3((unsigned)(x < most ? x : most), (unsigned)groups);
 }
 
+#define CXG_PR_LAUNCH_LANES(KERNEL, T, FMT)                                                                \
+  do {                                                                                                     \
+    if (pr_narrow(a.cols))                                                                                 \
+      hipLaunchKernelGGL((KERNEL<T, FMT, kPrLanesNarrow>), pack_grid(rows, 1, kPrThreads / kPrLanesNarrow), \
+                         dim3(kPrThreads), 0, st, a);                                                      \
+    else                                                                                                   \
+      hipLaunchKernelGGL((KERNEL<T, FMT, kPrLanes>), pack_grid(rows, a.groups, kPrThreads / kPrLanes),     \
+                         dim3(kPrThreads), 0, st, a);                                                      \
+  } while (0)
+#define CXG_PR_LAUNCH_FMT(KERNEL, T)                                                                       \
+  do {                                                                                                     \
+    if (fmt == CXG_PACK_INT8) CXG_PR_LAUNCH_LANES(KERNEL, T, CXG_PACK_INT8);                               \
+    else CXG_PR_LAUNCH_LANES(KERNEL, T, CXG_PACK_E4M3);                                                    \
+  } while (0)
 #define CXG_PR_LAUNCH(KERNEL, name)                                                                        \
   do {                                                                                                     \
-    const dim3 grid = pack_grid(rows, a.groups), block(kPrThreads);                                        \
-    const bool i8 = fmt == CXG_PACK_INT8;                                                                  \
-    if (type == CXG_F32) {                                                                                 \
-      if (i8) hipLaunchKernelGGL((KERNEL<float, CXG_PACK_INT8>), grid, block, 0, st, a);                   \
-      else hipLaunchKernelGGL((KERNEL<float, CXG_PACK_E4M3>), grid, block, 0, st, a);                      \
-    } else if (type == CXG_BF16) {                                                                         \
-      if (i8) hipLaunchKernelGGL((KERNEL<bf16_t, CXG_PACK_INT8>), grid, block, 0, st, a);                  \
-      else hipLaunchKernelGGL((KERNEL<bf16_t, CXG_PACK_E4M3>), grid, block, 0, st, a);                     \
-    } else {                                                                                               \
-      if (i8) hipLaunchKernelGGL((KERNEL<f16_t, CXG_PACK_INT8>), grid, block, 0, st, a);                   \
-      else hipLaunchKernelGGL((KERNEL<f16_t, CXG_PACK_E4M3>), grid, block, 0, st, a);                      \
-    }                                                                                                      \
+    if (type == CXG_F32) CXG_PR_LAUNCH_FMT(KERNEL, float);                                                 \
+    else if (type == CXG_BF16) CXG_PR_LAUNCH_FMT(KERNEL, bf16_t);                                          \
+    else CXG_PR_LAUNCH_FMT(KERNEL, f16_t);                                                                 \
     CXG_LAUNCH_CHECK(name);                                                                                \
   } while (0)
 

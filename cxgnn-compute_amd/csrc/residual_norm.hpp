@@ -126,6 +126,7 @@ __device__ __forceinline__ void team_sum(float (&v)[N], float (*s_red)[S::WAVES]
 // they fit) up to a team of 512 lanes.
 #define CXG_RN_WIDTH(F, TX, TF, TAIL)                                                      \
   do {                                                                                     \
+    if (a.cols <= 16) return F<TX, TF, 2, 8, TAIL>(a, st);                                 \
     if (a.cols <= 32) return F<TX, TF, 4, 8, TAIL>(a, st);                                 \
     if (a.cols <= 64) return F<TX, TF, 8, 8, TAIL>(a, st);                                 \
     if (a.cols <= 128) return F<TX, TF, 16, 8, TAIL>(a, st);                               \
@@ -141,7 +142,7 @@ __device__ __forceinline__ void team_sum(float (&v)[N], float (*s_red)[S::WAVES]
     constexpr int V = 16 / (int)sizeof(TX);                                                \
     if (a.cols % V == 0) CXG_RN_WIDTH(F, TX, TF, kRnWhole);                                \
     if (a.cols > V) CXG_RN_WIDTH(F, TX, TF, kRnShort);                                     \
-    return F<TX, TF, 4, 8, kRnTiny>(a, st);                                                \
+    return F<TX, TF, 2, 8, kRnTiny>(a, st);                                                \
   }
 #define CXG_RN_TYPES(F)                                                                    \
   CXG_RN_TYPE(F, CXG_F32, float, CXG_F32, float)                                           \

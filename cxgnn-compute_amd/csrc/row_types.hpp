@@ -40,7 +40,8 @@ template <int L> __device__ __forceinline__ float lanes_sum(float v) {
 // Sum over the lanes l, l + L, l + 2L, ... of the wave (same position in every group of L lanes).
 template <int L> __device__ __forceinline__ float groups_sum(float v) {
   typedef unsigned v2u __attribute__((ext_vector_type(2)));
-  static_assert(L >= 4, "groups of at least four lanes");
+  static_assert(L >= 2, "groups of at least two lanes");
+  if constexpr (L <= 2) v += __shfl_xor(v, 2, CXG_WAVE);
   if constexpr (L <= 4) v += __shfl_xor(v, 4, CXG_WAVE);
   if constexpr (L <= 8) v += __shfl_xor(v, 8, CXG_WAVE);
   if constexpr (L <= 16) {

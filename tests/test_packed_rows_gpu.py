@@ -91,7 +91,7 @@ def test_arguments_are_refused_on_the_host():
 @gpu
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
-@pytest.mark.parametrize("shape", [(1, 1), (5, 3), (33, 16), (70, 47), (64, 128), (31, 129), (9, 300), (257, 512), (3, 4100), (0, 8)])
+@pytest.mark.parametrize("shape", [(1, 1), (5, 3), (33, 16), (300, 32), (41, 33), (70, 47), (64, 128), (31, 129), (9, 300), (257, 512), (3, 4100), (0, 8)])
 def test_pack_and_unpack(shape, dtype, fmt):
     import cxgnncomp
     x = _rows(*shape, dtype=dtype, seed=shape[1])
