@@ -13,9 +13,9 @@
 // of four consecutive rows and writes, per column, the four rows as one 8-byte store into
 // [column][row] order (pitch 80 or 144 bytes).
 //
-// A block of four waves owns a 128 x 128 or 256 x 128 tile of gW over one chunk of a segment's rows, 64
-// or 32 rows per step: while the waves multiply a step from LDS the rows of the next one are on their
-// way into registers, and the two blocks of a CU cover each other's barriers.  128 columns of A are
+// A block of four waves owns a tile of gW (64 to 256 columns of A by 64 or 128 of G) over one chunk of a
+// segment's rows, 64 or 32 rows per step: while the waves multiply a step from LDS the rows of the next
+// one are on their way into registers, and the blocks of a CU cover each other's barriers.  128 columns of A are
 // one scale group.  Tiles of a chunk sit side by side on one die, whose L2 then holds the chunk's
 // rows for all of them.  Every block leaves its partial tile (and, if wanted, the sums of the rows of
 // G that pass through it, the bias gradient), a second kernel adds the chunks of a segment in order:
@@ -40,18 +40,16 @@ typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 
 constexpr int kPwThreads = 256;
 constexpr int kPwXcds = 8;               // accelerator dies, one L2 each
-constexpr int kPwTile = 128;             // columns of G of a tile, and of A per scale group
 constexpr int kPwFront = 8;              // columns in front of a tile of G: at least what a thread stages
-static_assert(kPwTile == kPrGroup, "one scale per row and 128 columns");
 
-// Shape of a block: KT columns of A, ROWS rows per step, BLOCKS of them per CU.
-template <int KT_, int ROWS_, int BLOCKS_> struct PwShape {
-  static constexpr int KT = KT_, ROWS = ROWS_, BLOCKS = BLOCKS_;
+// Shape of a block: KT columns of A, NT of G, ROWS rows per step, BLOCKS of them per CU.
+template <int KT_, int NT_, int ROWS_, int BLOCKS_> struct PwShape {
+  static constexpr int KT = KT_, NT = NT_, ROWS = ROWS_, BLOCKS = BLOCKS_;
   static constexpr int PITCH = ROWS + 8;                      // LDS pitch in bf16: 80 or 144 bytes
   static constexpr int MG = ROWS / 4;                         // groups of four rows
   static constexpr int CA = KT * ROWS / (4 * kPwThreads);     // columns of A / G that a thread stages
-  static constexpr int CG = kPwTile * ROWS / (4 * kPwThreads);
-  static constexpr int MI = KT / 64;                          // 32 x 32 blocks of a wave along K; two along N
+  static constexpr int CG = NT * ROWS / (4 * kPwThreads);
+  static constexpr int MI = KT / 64, NJ = NT / 64;            // 32 x 32 blocks of a wave along K and N
 };
 
 struct PwArgs {
@@ -107,17 +105,18 @@ __device__ __forceinline__ unsigned bf16_pair(float x, float y) {
 template <int FMT, typename TG, bool MAPPED, typename S, bool TINY>
 __global__ __launch_bounds__(kPwThreads, S::BLOCKS) void packed_wgrad_kernel(PwArgs a) {
   constexpr int NP = PwParts<TG>::value;
-  constexpr int ROWS = S::ROWS, MG = S::MG, CA = S::CA, CG = S::CG, MI = S::MI, PITCH = S::PITCH, NG = S::KT / kPrGroup;
+  constexpr int ROWS = S::ROWS, MG = S::MG, CA = S::CA, CG = S::CG, MI = S::MI, NJ = S::NJ, PITCH = S::PITCH;
+  constexpr int NG = (S::KT + kPrGroup - 1) / kPrGroup;                                   // scale groups of a tile
   __shared__ __attribute__((aligned(16))) uint16_t s_a[S::KT][PITCH];
-  __shared__ __attribute__((aligned(16))) uint16_t s_gp[NP][kPwFront + kPwTile][PITCH];   // kPwFront columns of slack in front
+  __shared__ __attribute__((aligned(16))) uint16_t s_gp[NP][kPwFront + S::NT][PITCH];   // kPwFront columns of slack in front
   __shared__ __attribute__((aligned(16))) uint8_t s_exp[2][NG][ROWS];                     // exponent bytes of a step's rows
   __shared__ int64_t s_off[MAPPED ? 3 : 1][2][MAPPED ? ROWS : 1];                         // ring: offsets of the rows of codes and g
   __shared__ unsigned long long s_live[3];                                                // and which of them are there
-  const int n_ct = (a.N + kPwTile - 1) / kPwTile, n_kt = (a.K + S::KT - 1) / S::KT, n_tile = n_ct * n_kt;
+  const int n_ct = (a.N + S::NT - 1) / S::NT, n_kt = (a.K + S::KT - 1) / S::KT, n_tile = n_ct * n_kt;
   const int64_t slot = blockIdx.x / kPwXcds;
   const int64_t chunk = (slot / n_tile) * kPwXcds + (blockIdx.x % kPwXcds);
   const int k0 = (int)((slot % n_tile) / n_ct) * S::KT;
-  const int n0 = (int)((slot % n_tile) % n_ct) * kPwTile;
+  const int n0 = (int)((slot % n_tile) % n_ct) * S::NT;
   int64_t row0 = 0, row_end = 0;
   if (chunk >= a.chunks || !pw_locate(a, chunk, row0, row_end)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform_i32(tid >> 6);
@@ -129,7 +128,7 @@ __global__ __launch_bounds__(kPwThreads, S::BLOCKS) void packed_wgrad_kernel(PwA
   // All loads of the loop are unconditional, so that none waits for another: columns of A past the
   // pitch read column k0, a piece of G that would pass N is moved back to end there (it then writes the
   // columns it shares with its neighbour twice, the same values, and those in front of the tile into the
-  // slack), rows that are not there read row 0 and are cleared when they are staged.  What is staged
+  // slack), rows that are not there read one that is and are cleared when they are staged.  What is staged
   // for columns of A or G that do not exist only reaches rows and columns of gW that do not exist.
   const int mg = lane % MG, cg = wave * (64 / MG) + lane / MG;
   const int ka = k0 + CA * cg;
@@ -138,12 +137,18 @@ __global__ __launch_bounds__(kPwThreads, S::BLOCKS) void packed_wgrad_kernel(PwA
   if (!TINY && ng + CG > a.N) ng = a.N - CG;                    // N >= CG
   const int gcol = TINY ? kPwFront + CG * cg : kPwFront + ng - n0 < 0 ? 0 : kPwFront + ng - n0;
   const TG* const g_base = static_cast<const TG*>(a.g) + (TINY ? 0 : ng);
-  // exponent bytes: lane of the first wave -> (group, row)
-  const int e_grp = (k0 / kPrGroup + lane / ROWS) < a.groups ? k0 / kPrGroup + lane / ROWS : a.groups - 1;
+  // exponent bytes: lane of the first wave -> row and NE groups
+  constexpr int NE = (NG * ROWS + 63) / 64;
+  int e_grp[NE];
+#pragma unroll
+  for (int j = 0; j < NE; ++j) {
+    e_grp[j] = k0 / kPrGroup + lane / ROWS + j;
+    e_grp[j] = e_grp[j] < a.groups ? e_grp[j] : a.groups - 1;
+  }
   unsigned code[4][CA / 4];
   TG gv[4][CG];
-  unsigned expo = 0;
-  static_assert(NG * ROWS <= 64, "one exponent byte per lane");
+  unsigned expo[NE] = {};
+  static_assert(ROWS <= 64 && (NE == 1 || ROWS == 64), "a lane per row, or per row and group");
 
   auto load_row = [&](int i, int64_t oa, int64_t og) {
     typedef unsigned piece_t __attribute__((ext_vector_type(CA / 4)));
@@ -186,28 +191,37 @@ __global__ __launch_bounds__(kPwThreads, S::BLOCKS) void packed_wgrad_kernel(PwA
     return ok ? ia * a.groups : 0;
   };
   // rows of step t into registers; behind the last step the last one again
+  const int64_t a_off = (int64_t)(4 * mg) * a.pitch, g_off = (int64_t)(4 * mg) * a.ldg;
   auto load = [&](int t, int64_t off_exp) {
     t = t < steps ? t : steps - 1;
     const int64_t first = row0 + (int64_t)t * ROWS;
+    const int left = t + 1 < steps ? ROWS : last_rows;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (MAPPED) {
         load_row(i, s_off[t % 3][0][4 * mg + i], s_off[t % 3][1][4 * mg + i]);
       } else {
-        const int64_t r = first + 4 * mg + i < row_end ? first + 4 * mg + i : row0;
-        load_row(i, r * a.pitch, r * a.ldg);
+        // row first + 4 mg + i, or first + i, or first.  (A vector multiplication per row and step, the plain
+        // form of this, costs as much as decoding A.)
+        const bool on = 4 * mg + i < left;
+        const int64_t near = first + (i < left ? i : 0);
+        load_row(i, near * a.pitch + (on ? a_off : 0), near * a.ldg + (on ? g_off : 0));
       }
     }
     if (wave == 0) {
       if constexpr (!MAPPED) {
         const int row = lane & (ROWS - 1);
-        off_exp = (first + row < row_end ? first + row : row0) * a.groups;
+        off_exp = (first + (row < left ? row : 0)) * a.groups;
       }
-      expo = a.exps[off_exp + e_grp];
+#pragma unroll
+      for (int j = 0; j < NE; ++j) expo[j] = a.exps[off_exp + e_grp[j]];
     }
   };
   auto put_exp = [&](int t) {
-    if (wave == 0 && lane < NG * ROWS) s_exp[t & 1][lane / ROWS][lane & (ROWS - 1)] = (uint8_t)expo;
+    if (wave == 0 && lane < NG * ROWS) {
+#pragma unroll
+      for (int j = 0; j < NE; ++j) s_exp[t & 1][lane / ROWS + j][lane & (ROWS - 1)] = (uint8_t)expo[j];
+    }
   };
   const bool sums = a.stride > (int64_t)a.K * a.N && k0 == 0;    // this block also adds up the rows of its columns of G
   float colsum[CG];
@@ -278,12 +292,12 @@ __global__ __launch_bounds__(kPwThreads, S::BLOCKS) void packed_wgrad_kernel(PwA
     }
   };
 
-  const int wk = (wave >> 1) * (S::KT / 2), wn = (wave & 1) * 64;
-  v16f acc[MI][2];
+  const int wk = (wave >> 1) * (S::KT / 2), wn = (wave & 1) * (S::NT / 2);
+  v16f acc[MI][NJ];
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < NJ; ++j)
 #pragma unroll
       for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
   const bool active = k0 + wk < a.K && n0 + wn < a.N;           // else nothing of this wave's part lies inside gW
@@ -320,19 +334,19 @@ __global__ __launch_bounds__(kPwThreads, S::BLOCKS) void packed_wgrad_kernel(PwA
     for (int ms = 0; ms < ROWS / 16; ++ms) {
       if (!active) break;
       const int m = ms * 16 + (lane >> 5) * 8;
-      v8bf fa[MI], fg[NP][2];
+      v8bf fa[MI], fg[NP][NJ];
 #pragma unroll
       for (int i = 0; i < MI; ++i) fa[i] = *reinterpret_cast<const v8bf*>(&s_a[wk + 32 * i + (lane & 31)][m]);
 #pragma unroll
       for (int p = NP - 1; p >= 0; --p)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) fg[p][j] = *reinterpret_cast<const v8bf*>(&s_gp[p][kPwFront + wn + 32 * j + (lane & 31)][m]);
+        for (int j = 0; j < NJ; ++j) fg[p][j] = *reinterpret_cast<const v8bf*>(&s_gp[p][kPwFront + wn + 32 * j + (lane & 31)][m]);
 #pragma unroll
       for (int p = NP - 1; p >= 0; --p)                  // the small parts first
 #pragma unroll
         for (int i = 0; i < MI; ++i)
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int j = 0; j < NJ; ++j)
             acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fg[p][j], acc[i][j], 0, 0, 0);
     }
     __builtin_amdgcn_s_setprio(0);
@@ -340,13 +354,13 @@ __global__ __launch_bounds__(kPwThreads, S::BLOCKS) void packed_wgrad_kernel(PwA
   float* const part = a.partial + (size_t)chunk * (size_t)a.stride;
   if (sums) {
     // over the groups of four rows, through the LDS that held G (a column that two threads hold, they hold alike)
-    float (*const s_sum)[kPwFront + kPwTile] = reinterpret_cast<float (*)[kPwFront + kPwTile]>(&s_gp[0][0][0]);
-    static_assert(sizeof(float) * MG * (kPwFront + kPwTile) <= sizeof(s_gp), "the sums fit");
+    float (*const s_sum)[kPwFront + S::NT] = reinterpret_cast<float (*)[kPwFront + S::NT]>(&s_gp[0][0][0]);
+    static_assert(sizeof(float) * MG * (kPwFront + S::NT) <= sizeof(s_gp), "the sums fit");
     __syncthreads();
 #pragma unroll
     for (int c = 0; c < CG; ++c) s_sum[mg][gcol + c] = colsum[c];
     __syncthreads();
-    if (tid < kPwTile && n0 + tid < a.N) {
+    if (tid < S::NT && n0 + tid < a.N) {
       float v = 0.f;
 #pragma unroll
       for (int q = 0; q < MG; ++q) v += s_sum[q][kPwFront + tid];
@@ -356,7 +370,7 @@ __global__ __launch_bounds__(kPwThreads, S::BLOCKS) void packed_wgrad_kernel(PwA
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < NJ; ++j) {
       const int col = n0 + wn + 32 * j + (lane & 31);
 #pragma unroll
       for (int q = 0; q < 16; ++q) {
@@ -404,25 +418,40 @@ __global__ __launch_bounds__(256) void packed_wgrad_sums_kernel(PwArgs a, float*
 
 // Inputs of at most 128 columns: 128 x 128 tiles, 64 rows per step, two blocks per CU (32 rows and three
 // blocks: 114 against 97 us for 1 M rows x 128 x 128 of 16 types in bf16, 55 against 50 us for 169,343 x
-// 128 x 256 in fp32; this kernel alone).  Wider inputs: 256 x 128 tiles, so that a step of G is staged once per 256 columns
-// of A (2.33 M x 512 x 512 in fp32).
-typedef PwShape<128, 64, 2> PwNarrow;
-typedef PwShape<256, 32, 2> PwWide;
+// 128 x 256 in fp32; this kernel alone).  Wider inputs: 256 x 128 tiles, so that a step of G is staged once
+// per 256 columns of A (2.33 M x 512 x 512 in fp32: 3.6 ms; 512 x 128 tiles of one block of eight waves per
+// CU, staging into a second buffer while the other half multiplies: 4.1 ms).  At most 64 columns of G: tiles
+// of 64, which leave room for more rows on their way (2.45 M x 256 x 47 in fp32 390 -> 290 us, 1 M x 64 x 8
+// 94 -> 67 us, against 128).
+typedef PwShape<64, 64, 64, 3> PwSmall;
+typedef PwShape<128, 64, 64, 3> PwNarrowFew;
+typedef PwShape<256, 64, 64, 2> PwWideFew;
+typedef PwShape<128, 128, 64, 2> PwNarrow;
+typedef PwShape<256, 128, 32, 2> PwWide;
 
-bool pw_wide(int K) { return K > kPwTile; }
+// run(shape) with the shape for K columns of A and N of G
+template <typename F> auto pw_shaped(int K, int N, F run) {
+  if (N <= 64) return K <= 64 ? run(PwSmall{}) : K <= 128 ? run(PwNarrowFew{}) : run(PwWideFew{});
+  return K <= 128 ? run(PwNarrow{}) : run(PwWide{});
+}
 
 // Rows per chunk: one round of blocks on the chip where a chunk is short (its partial tile is written
 // and read again, which a chunk should outweigh), up to two rounds where it is long (a last round
-// that is not full then costs little).  A segment's last chunk is ragged: R of them per tile.
-int64_t pw_tiles(int K, int N) { return ceil_div(K, pw_wide(K) ? PwWide::KT : kPwTile) * ceil_div(N, kPwTile); }
+// that is not full then costs little).  The tiles of a chunk run on one die: a round is full with as many
+// chunks as fit on each die whole, the same number everywhere, the ragged last chunks of the segments among
+// them (30,289 x 529 x 505 of 3 types, 12 tiles, in bf16: 42 chunks, six on two of the dies, 108 us; 40
+// chunks, five on each, 76 us).
+int64_t pw_tiles(int K, int N) {
+  return pw_shaped(K, N, [&](auto s) { return ceil_div(K, s.KT) * ceil_div(N, s.NT); });
+}
 
 int64_t pw_chunk_rows(int64_t M, int K, int N, int R) {
   const int64_t tiles = pw_tiles(K, N);
-  const int64_t slots = 256 * (pw_wide(K) ? PwWide::BLOCKS : PwNarrow::BLOCKS);
+  const int64_t slots = 256 / kPwXcds * pw_shaped(K, N, [](auto s) { return (int64_t)s.BLOCKS; });   // of one die
   auto fill = [&](int64_t rounds) {                       // rows so that about `rounds` rounds are full
-    int64_t chunks = ceil_div(slots * rounds, tiles) - R;
-    if (chunks < 1) chunks = 1;
-    return ceil_div(M, chunks);
+    const int64_t each = slots * rounds / tiles;          // chunks per die
+    const int64_t chunks = kPwXcds * (each < 1 ? 1 : each) - (R - 1);
+    return ceil_div(M, chunks < 1 ? 1 : chunks);
   };
   const int64_t longest = fill(1), shortest = fill(2);
   int64_t rows = 2048;
@@ -431,24 +460,30 @@ int64_t pw_chunk_rows(int64_t M, int K, int N, int R) {
 }
 
 int64_t pw_chunk_count(int64_t M, int K, int N, int R) {
-  return ceil_div(ceil_div(M, pw_chunk_rows(M, K, N, R)) + R, kPwXcds) * kPwXcds;
+  return ceil_div(ceil_div(M, pw_chunk_rows(M, K, N, R)) + R - 1, kPwXcds) * kPwXcds;
 }
 
 template <int FMT, typename TG, typename S, bool TINY> void pw_launch(const PwArgs& a, int64_t chunks, hipStream_t st) {
-  const int64_t tiles = ceil_div(a.K, S::KT) * ceil_div(a.N, kPwTile);
+  const int64_t tiles = ceil_div(a.K, S::KT) * ceil_div(a.N, S::NT);
   const dim3 grid((unsigned)(chunks * tiles)), block(kPwThreads);
   static_assert(S::CG <= kPwFront, "the slack in front of a tile of G");
   if (a.src || a.dst) hipLaunchKernelGGL((packed_wgrad_kernel<FMT, TG, true, S, TINY>), grid, block, 0, st, a);
   else hipLaunchKernelGGL((packed_wgrad_kernel<FMT, TG, false, S, TINY>), grid, block, 0, st, a);
 }
 template <int FMT, typename TG> void pw_launch_shape(const PwArgs& a, int64_t chunks, hipStream_t st) {
-  if (pw_wide(a.K)) {
-    if (a.N < PwWide::CG) pw_launch<FMT, TG, PwWide, true>(a, chunks, st);
-    else pw_launch<FMT, TG, PwWide, false>(a, chunks, st);
-  } else {
-    if (a.N < PwNarrow::CG) pw_launch<FMT, TG, PwNarrow, true>(a, chunks, st);
-    else pw_launch<FMT, TG, PwNarrow, false>(a, chunks, st);
-  }
+  pw_shaped(a.K, a.N, [&](auto s) {
+    // 64 rows per step wherever the LDS of a CU then holds BLOCKS blocks (all but 256 x 128 in fp32): half the
+    // barriers and loads twice as far apart (300,000 x 1,024 x 1,024 in bf16 1,103 -> 770 us, in fp16 1,334 -> 1,135 us
+    // against 32 rows)
+    using W = decltype(s);
+    constexpr int NP = PwParts<TG>::value;
+    constexpr int lds64 = (W::KT + NP * (kPwFront + W::NT)) * 2 * (64 + 8) + 3500;    // tiles; maps and exponent bytes
+    using S = PwShape<W::KT, W::NT, lds64 * W::BLOCKS <= 160 * 1024 ? 64 : W::ROWS, W::BLOCKS>;
+    if constexpr (S::NT <= 64) {
+      if (a.N < S::CG) return pw_launch<FMT, TG, S, true>(a, chunks, st);
+    }
+    pw_launch<FMT, TG, S, false>(a, chunks, st);
+  });
 }
 template <int FMT> void pw_launch_type(const PwArgs& a, int g_type, int64_t chunks, hipStream_t st) {
   if (g_type == CXG_F32) pw_launch_shape<FMT, float>(a, chunks, st);

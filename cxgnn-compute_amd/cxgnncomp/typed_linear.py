@@ -103,6 +103,8 @@ class TypedLinearE2EOP(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_out):
+        if ctx.checkpoint is not None and torch.is_grad_enabled():
+            raise RuntimeError("TypedLinearE2EOP(checkpoint=) has no second derivatives (create_graph=True)")
         weights, types, indices, sorted_types, *kept = ctx.saved_tensors
         grad_out = grad_out.contiguous()
         grad_x = grad_w = None

@@ -198,7 +198,7 @@ def _wgrad(case, k, fmt, with_seg=True):
 
 
 @gpu
-@pytest.mark.parametrize("k,n", [(1, 1), (16, 3), (47, 64), (128, 128), (129, 47), (96, 160), (300, 130), (512, 256)])
+@pytest.mark.parametrize("k,n", [(1, 1), (16, 3), (47, 64), (128, 128), (129, 47), (96, 160), (300, 130), (512, 256), (64, 64), (65, 65), (60, 3), (100, 1), (129, 64), (200, 1), (513, 2)])
 @pytest.mark.parametrize("fmt,dtype", [("int8", F32), ("int8", BF16), ("int8", F16), ("e4m3", F32), ("e4m3", BF16), ("e4m3", F16)])
 def test_weight_grad_shapes(k, n, fmt, dtype):
     for m in (33, 700):
