@@ -97,6 +97,20 @@ template <typename S> struct RnPieces {
   }
 };
 
+// The rows of a block's teams: the first row of this wave, the same for all its lanes, and what the lane's
+// team adds to it.  (A row number per lane costs a 64-bit vector multiplication per tensor and row, a fifth
+// of what the forward pass computes for a narrow row.)
+template <typename S> struct RnRow {
+  int wave_team, lane_team;
+  int64_t first = 0;                                      // row of the wave's first team
+  __device__ __forceinline__ RnRow() {
+    wave_team = S::L < CXG_WAVE ? uniform_i32(threadIdx.x >> 6) * (CXG_WAVE / S::L) : uniform_i32(threadIdx.x / S::L);
+    lane_team = S::L < CXG_WAVE ? (int)(threadIdx.x & (CXG_WAVE - 1)) / S::L : 0;
+  }
+  __device__ __forceinline__ int64_t row() const { return first + lane_team; }
+  template <typename T> __device__ __forceinline__ T* of(T* p, int64_t ld) const { return p + first * ld + lane_team * ld; }
+};
+
 // Sum over the team; every lane gets it.  Teams of several waves meet in LDS (`slot` alternates between
 // two buffers, so that one barrier per sum is enough).
 template <typename S, int N>

@@ -27,13 +27,14 @@ namespace {
 constexpr int kRnMaxBlocks = 768;        // partial rows; three blocks of 256 threads per CU are resident
 
 template <typename TX, typename TF, typename S>
-__global__ __launch_bounds__(S::THREADS) void residual_norm_bwd_kernel(RnArgs a) {
+__global__ __launch_bounds__(S::THREADS, S::THREADS == 256 ? 3 : 2) void residual_norm_bwd_kernel(RnArgs a) {
   constexpr int L = S::L, V = S::V, ITEMS = S::ITEMS, kTeams = S::TEAMS;
   __shared__ float s_red[2][S::WAVES][2];
-  const int lit = threadIdx.x % L, team = threadIdx.x / L;
+  const int lit = threadIdx.x % L;
   const int cols = a.cols;
   const float inv_c = 1.0f / (float)cols;
   const RnPieces<S> at(cols);
+  RnRow<S> of_row;
   int slot = 0;
   const bool post = a.post_kind != CXG_NORM_NONE, pre = a.pre_kind != CXG_NORM_NONE;
   const bool post_layer = a.post_kind == CXG_NORM_LAYER, pre_layer = a.pre_kind == CXG_NORM_LAYER;
@@ -52,9 +53,8 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_bwd_kernel(RnArgs a)
       for (int j = 0; j < V; ++j) sums[q][i][j] = 0.f;
 
   for (int64_t base = (int64_t)blockIdx.x * kTeams; base < a.rows; base += (int64_t)gridDim.x * kTeams) {
-    const int64_t row = base + team;
-    const bool live = row < a.rows;
-    const int64_t rr = live ? row : 0;
+    of_row.first = base + of_row.wave_team;
+    const bool live = of_row.row() < a.rows;
     RowPiece<TX, V> px[ITEMS], pdr[ITEMS];
     RowPiece<TF, V> pf[ITEMS], pg[ITEMS], pdy[ITEMS];
     const bool full = a.gate_kind == CXG_GATE_FULL;
@@ -62,15 +62,15 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_bwd_kernel(RnArgs a)
     for (int i = 0; i < ITEMS; ++i) {                     // a row that does not exist adds zeros everywhere
       pf[i].t = pg[i].t = pdy[i].t = (TF)0.f;
       pdr[i].t = (TX)0.f;
-      at.load(px[i], static_cast<const TX*>(a.x) + rr * a.ldx, i, live);
-      if (a.f) at.load(pf[i], static_cast<const TF*>(a.f) + rr * a.ldf, i, live);
-      if (a.dr) at.load(pdr[i], static_cast<const TX*>(a.dr) + rr * a.lddr, i, live);
-      if (a.dy) at.load(pdy[i], static_cast<const TF*>(a.dy) + rr * a.lddy, i, live);
-      if (full) at.load(pg[i], static_cast<const TF*>(a.gate) + rr * a.ldg, i, live);
+      at.load(px[i], of_row.of(static_cast<const TX*>(a.x), a.ldx), i, live);
+      if (a.f) at.load(pf[i], of_row.of(static_cast<const TF*>(a.f), a.ldf), i, live);
+      if (a.dr) at.load(pdr[i], of_row.of(static_cast<const TX*>(a.dr), a.lddr), i, live);
+      if (a.dy) at.load(pdy[i], of_row.of(static_cast<const TF*>(a.dy), a.lddy), i, live);
+      if (full) at.load(pg[i], of_row.of(static_cast<const TF*>(a.gate), a.ldg), i, live);
     }
-    const float grow = a.gate_kind == CXG_GATE_ROW && live ? (float)static_cast<const TF*>(a.gate)[rr * a.ldg] : 1.f;
+    const float grow = a.gate_kind == CXG_GATE_ROW && live ? (float)*of_row.of(static_cast<const TF*>(a.gate), a.ldg) : 1.f;
     float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
-    if (live) st = reinterpret_cast<const float4*>(a.stats)[rr];
+    if (live) st = *of_row.of(reinterpret_cast<const float4*>(a.stats), 1);
 
     float fh[ITEMS][V], h[ITEMS][V], gt[ITEMS][V], rh[ITEMS][V], g[ITEMS][V];
     float s[2] = {0.f, 0.f};
@@ -110,7 +110,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_bwd_kernel(RnArgs a)
       }
     }
     if (a.dx && live) {
-      TX* const out = static_cast<TX*>(a.dx) + rr * cols;
+      TX* const out = of_row.of(static_cast<TX*>(a.dx), cols);
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
         float o[V];
@@ -122,7 +122,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_bwd_kernel(RnArgs a)
     if (a.dgate) {
       if (full) {
         if (live) {
-          TF* const out = static_cast<TF*>(a.dgate) + rr * cols;
+          TF* const out = of_row.of(static_cast<TF*>(a.dgate), cols);
 #pragma unroll
           for (int i = 0; i < ITEMS; ++i) {
             float o[V];
@@ -138,7 +138,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_bwd_kernel(RnArgs a)
 #pragma unroll
           for (int j = 0; j < V; ++j) d[0] += at.counts(i, j) ? g[i][j] * h[i][j] : 0.f;
         team_sum<S, 1>(d, s_red, slot);
-        if (live && lit == 0) static_cast<TF*>(a.dgate)[rr] = (TF)(a.branch_scale * d[0]);
+        if (live && lit == 0) *of_row.of(static_cast<TF*>(a.dgate), 1) = (TF)(a.branch_scale * d[0]);
       }
     }
     if (a.f) {
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_bwd_kernel(RnArgs a)
           m1 = q[1] * inv_c;
         }
         if (live) {
-          TF* const out = static_cast<TF*>(a.df) + rr * cols;
+          TF* const out = of_row.of(static_cast<TF*>(a.df), cols);
 #pragma unroll
           for (int i = 0; i < ITEMS; ++i) {
             float o[V];
@@ -192,7 +192,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_bwd_kernel(RnArgs a)
   } else {
     constexpr int kParts = L < CXG_WAVE ? S::WAVES : kTeams;     // waves, or teams of whole waves
     __shared__ float s_col[kParts][L * S::PER];
-    const int part = L < CXG_WAVE ? (int)(threadIdx.x >> 6) : team;
+    const int part = L < CXG_WAVE ? (int)(threadIdx.x >> 6) : of_row.wave_team;
 #pragma unroll
     for (int q = 0; q < kRnSums; ++q) {
       if (q) __syncthreads();

@@ -49,10 +49,11 @@ template <typename TX, typename TF, typename S>
 __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a) {
   constexpr int L = S::L, V = S::V, ITEMS = S::ITEMS, kTeams = S::TEAMS;
   __shared__ float s_red[2][S::WAVES][2];
-  const int lit = threadIdx.x % L, team = threadIdx.x / L;
+  const int lit = threadIdx.x % L;
   const int cols = a.cols;
   const float inv_c = 1.0f / (float)cols;
   const RnPieces<S> at(cols);
+  RnRow<S> of_row;
   int slot = 0;
   float w1[ITEMS][V], b1[ITEMS][V], w2[ITEMS][V], b2[ITEMS][V], gc[ITEMS][V];
   if (a.post_kind != CXG_NORM_NONE) {
@@ -67,26 +68,25 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a)
 
   // every lane stays in the loop as long as its block: the reductions need whole waves
   for (int64_t base = (int64_t)blockIdx.x * kTeams; base < a.rows; base += (int64_t)gridDim.x * kTeams) {
-    const int64_t row = base + team;
-    const bool live = row < a.rows;
-    const int64_t rr = live ? row : 0;
+    of_row.first = base + of_row.wave_team;
+    const bool live = of_row.row() < a.rows;
     RowPiece<TX, V> px[ITEMS];
     RowPiece<TF, V> pf[ITEMS], pg[ITEMS];
-    const TX* const xrow = static_cast<const TX*>(a.x) + rr * a.ldx;
+    const TX* const xrow = of_row.of(static_cast<const TX*>(a.x), a.ldx);
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) at.load(px[i], xrow, i);
+    for (int i = 0; i < ITEMS; ++i) at.load(px[i], xrow, i, live);
     if (a.f) {
-      const TF* const frow = static_cast<const TF*>(a.f) + rr * a.ldf;
+      const TF* const frow = of_row.of(static_cast<const TF*>(a.f), a.ldf);
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i) at.load(pf[i], frow, i);
+      for (int i = 0; i < ITEMS; ++i) at.load(pf[i], frow, i, live);
     }
     float grow = 1.f;
     if (a.gate_kind == CXG_GATE_FULL) {
-      const TF* const gr = static_cast<const TF*>(a.gate) + rr * a.ldg;
+      const TF* const gr = of_row.of(static_cast<const TF*>(a.gate), a.ldg);
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i) at.load(pg[i], gr, i);
-    } else if (a.gate_kind == CXG_GATE_ROW) {
-      grow = (float)static_cast<const TF*>(a.gate)[rr * a.ldg];
+      for (int i = 0; i < ITEMS; ++i) at.load(pg[i], gr, i, live);
+    } else if (a.gate_kind == CXG_GATE_ROW && live) {
+      grow = (float)*of_row.of(static_cast<const TF*>(a.gate), a.ldg);
     }
 
     float v[ITEMS][V];                               // the branch row, then the stream row
@@ -114,7 +114,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a)
             s[0] += at.counts(i, j) ? v[i][j] * v[i][j] : 0.f;
           }
         team_sum<S, 1>(s, s_red, slot);
-        rstd1 = 1.0f / sqrtf(s[0] * inv_c + a.eps);
+        rstd1 = inverse_sqrt(s[0] * inv_c + a.eps);
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
@@ -152,7 +152,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a)
       }
     }
     if (a.r && live) {
-      TX* const out = static_cast<TX*>(a.r) + rr * cols;
+      TX* const out = of_row.of(static_cast<TX*>(a.r), cols);
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) at.store(v[i], out, i);
     }
@@ -176,9 +176,9 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a)
           s[0] += at.counts(i, j) ? v[i][j] * v[i][j] : 0.f;
         }
       team_sum<S, 1>(s, s_red, slot);
-      rstd2 = 1.0f / sqrtf(s[0] * inv_c + a.eps);
+      rstd2 = inverse_sqrt(s[0] * inv_c + a.eps);
       if (live) {
-        TF* const out = static_cast<TF*>(a.y) + rr * cols;
+        TF* const out = of_row.of(static_cast<TF*>(a.y), cols);
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
           float o[V];
@@ -189,7 +189,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a)
       }
     }
     if (a.stats && live && lit == 0)
-      reinterpret_cast<float4*>(a.stats)[row] = make_float4(mean1, rstd1, mean2, rstd2);
+      *of_row.of(reinterpret_cast<float4*>(a.stats), 1) = make_float4(mean1, rstd1, mean2, rstd2);
   }
 }
 
