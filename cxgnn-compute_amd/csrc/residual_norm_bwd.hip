@@ -17,6 +17,8 @@
 // dgate = b * (w_post * sum g * fhat + b_post * sum g) needs no sum of its own.  Teams of a block meet
 // in registers and LDS, blocks leave one partial row each, a second kernel adds the partial rows in
 // block order: no atomics, and the grid depends on the shape alone, so results repeat bit for bit.
+// b * channel gate * (w_post, b_post) is formed once per column: a third fewer operations per value and 16
+// registers less (48 M values in rows of 8,192: bf16 181 -> 139 us, fp32 241 -> 220 us).
 // Measured: 169,343 x 256 fp32, channel gate 211 us = 4.9 TB/s; 2,449,029 x 128 bf16, element gate
 // 1.02 ms = 4.9 TB/s; the second kernel 9 us.
 #include "residual_norm.hpp"
@@ -38,12 +40,21 @@ __global__ __launch_bounds__(S::THREADS, S::THREADS == 256 ? 3 : 2) void residua
   int slot = 0;
   const bool post = a.post_kind != CXG_NORM_NONE, pre = a.pre_kind != CXG_NORM_NONE;
   const bool post_layer = a.post_kind == CXG_NORM_LAYER, pre_layer = a.pre_kind == CXG_NORM_LAYER;
-  float w1[ITEMS][V], b1[ITEMS][V], w2[ITEMS][V], gc[ITEMS][V];
-  // columns that do not exist have weight 0 and so add nothing to the sums over a row
+  // what is the same for all rows, b * channel gate * (w_post, b_post) and w_pre, per column; columns that do
+  // not exist have weight 0 and so add nothing to the sums over a row
+  float w1[ITEMS][V], b1[ITEMS][V], w2[ITEMS][V];
   at.params(post ? a.post_w : nullptr, 1.f, w1);
   at.params(post ? a.post_b : nullptr, 0.f, b1);
+  at.params(a.gate_kind == CXG_GATE_CHANNEL ? static_cast<const float*>(a.gate) : nullptr, 1.f, w2);
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float scale = a.branch_scale * w2[i][j];
+      w1[i][j] *= scale;
+      b1[i][j] *= scale;
+    }
   at.params(pre ? a.pre_w : nullptr, 1.f, w2);
-  at.params(a.gate_kind == CXG_GATE_CHANNEL ? static_cast<const float*>(a.gate) : nullptr, 1.f, gc);
   float sums[kRnSums][ITEMS][V];
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i)
@@ -72,26 +83,26 @@ __global__ __launch_bounds__(S::THREADS, S::THREADS == 256 ? 3 : 2) void residua
     float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
     if (live) st = *of_row.of(reinterpret_cast<const float4*>(a.stats), 1);
 
-    float fh[ITEMS][V], h[ITEMS][V], gt[ITEMS][V], rh[ITEMS][V], g[ITEMS][V];
+    // the normalised rows, b * channel gate * h, the gate as far as it differs between rows, t, the gradient of r
+    float fh[ITEMS][V], h[ITEMS][V], gt[ITEMS][V], rh[ITEMS][V], t[ITEMS][V], g[ITEMS][V];
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      float x[V], f[V], dy[V], gf[V];
+      float x[V], f[V], dy[V];
       px[i].widen(x);
       pf[i].widen(f);
       pdy[i].widen(dy);
-      pg[i].widen(gf);
+      pg[i].widen(gt[i]);
       pdr[i].widen(g[i]);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        fh[i][j] = post ? (f[j] - st.x) * st.y : f[j];
-        h[i][j] = post ? fh[i][j] * w1[i][j] + b1[i][j] : f[j];
-        gt[i][j] = full ? gf[j] : grow;                 // the gate as far as it differs between rows
-        const float hg = (full ? h[i][j] * gf[j] : h[i][j] * gc[i][j]);
-        const float r = a.res_scale * x[j] + a.branch_scale * grow * hg;
+        fh[i][j] = (f[j] - st.x) * st.y;                // (mean 0 and 1/std 1 without a norm)
+        h[i][j] = fh[i][j] * w1[i][j] + b1[i][j];
+        gt[i][j] = full ? gt[i][j] : grow;
+        const float r = a.res_scale * x[j] + gt[i][j] * h[i][j];
         rh[i][j] = (r - st.z) * st.w;
-        const float t = dy[j] * w2[i][j];
-        const float tc = S::TAIL != kRnShort || at.counts(i, j) ? t : 0.f;
+        t[i][j] = dy[j] * w2[i][j];
+        const float tc = S::TAIL != kRnShort || at.counts(i, j) ? t[i][j] : 0.f;
         s[0] += tc;
         s[1] += tc * rh[i][j];
         sums[0][i][j] += dy[j] * rh[i][j];
@@ -102,12 +113,9 @@ __global__ __launch_bounds__(S::THREADS, S::THREADS == 256 ? 3 : 2) void residua
       team_sum<S, 2>(s, s_red, slot);
       const float m0 = pre_layer ? s[0] * inv_c : 0.f, m1 = s[1] * inv_c;
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i) {
-        float dy[V];
-        pdy[i].widen(dy);
+      for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) g[i][j] += st.w * (dy[j] * w2[i][j] - m0 - rh[i][j] * m1);
-      }
+        for (int j = 0; j < V; ++j) g[i][j] += st.w * (t[i][j] - m0 - rh[i][j] * m1);
     }
     if (a.dx && live) {
       TX* const out = of_row.of(static_cast<TX*>(a.dx), cols);
@@ -127,7 +135,7 @@ __global__ __launch_bounds__(S::THREADS, S::THREADS == 256 ? 3 : 2) void residua
           for (int i = 0; i < ITEMS; ++i) {
             float o[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) o[j] = a.branch_scale * g[i][j] * h[i][j];
+            for (int j = 0; j < V; ++j) o[j] = g[i][j] * h[i][j];
             at.store(o, out, i);
           }
         }
@@ -138,7 +146,7 @@ __global__ __launch_bounds__(S::THREADS, S::THREADS == 256 ? 3 : 2) void residua
 #pragma unroll
           for (int j = 0; j < V; ++j) d[0] += at.counts(i, j) ? g[i][j] * h[i][j] : 0.f;
         team_sum<S, 1>(d, s_red, slot);
-        if (live && lit == 0) *of_row.of(static_cast<TF*>(a.dgate), 1) = (TF)(a.branch_scale * d[0]);
+        if (live && lit == 0) *of_row.of(static_cast<TF*>(a.dgate), 1) = (TF)d[0];
       }
     }
     if (a.f) {
@@ -147,10 +155,10 @@ __global__ __launch_bounds__(S::THREADS, S::THREADS == 256 ? 3 : 2) void residua
       for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const float cg = live ? gt[i][j] * g[i][j] : 0.f;
+          const float cg = gt[i][j] * g[i][j];          // (0 in a row that does not exist)
           sums[2][i][j] += cg * fh[i][j];
           sums[3][i][j] += cg;
-          g[i][j] = a.branch_scale * cg * (full ? 1.f : gc[i][j]) * w1[i][j];
+          g[i][j] = cg * w1[i][j];
           const float gc_ = S::TAIL != kRnShort || at.counts(i, j) ? g[i][j] : 0.f;
           q[0] += gc_;
           q[1] += gc_ * fh[i][j];

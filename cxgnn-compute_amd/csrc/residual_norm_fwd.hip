@@ -14,8 +14,8 @@
 // deviations from the registers, so a mean far from zero costs no digits.  A team of lanes owns a row,
 // 8 columns per lane whatever the width: the vectors of the norms then stay in registers from row to row
 // and enough waves fit a CU to keep memory busy.  (Up to 32 columns per lane left rows of 512 bf16 columns
-// at 1.2 TB/s; a grid of more blocks than are resident loads the vectors more often, 3.6 against 5.1 TB/s.)  Rows start at any value: the 16-byte
-// accesses assume the alignment of one value only.  Measured: 169,343 x 256 fp32, channel gate 124 us =
+// at 1.2 TB/s; a grid of more blocks than are resident loads the vectors more often, 3.6 against 5.1 TB/s.)  Rows
+// start at any value: the 16-byte accesses assume the alignment of one value only.  Measured: 169,343 x 256 fp32, channel gate 124 us =
 // 5.6 TB/s; 2,449,029 x 128 bf16, element gate 645 us = 4.9 TB/s.
 #include "residual_norm.hpp"
 
@@ -46,7 +46,7 @@ int rn_check(const RnArgs& a, int stream_type, int branch_type) {
 namespace {
 
 template <typename TX, typename TF, typename S>
-__global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a) {
+__global__ __launch_bounds__(S::THREADS, S::THREADS == 256 ? 5 : S::PER == 8 ? 4 : 2) void residual_norm_fwd_kernel(RnArgs a) {
   constexpr int L = S::L, V = S::V, ITEMS = S::ITEMS, kTeams = S::TEAMS;
   __shared__ float s_red[2][S::WAVES][2];
   const int lit = threadIdx.x % L;
@@ -55,16 +55,24 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a)
   const RnPieces<S> at(cols);
   RnRow<S> of_row;
   int slot = 0;
-  float w1[ITEMS][V], b1[ITEMS][V], w2[ITEMS][V], b2[ITEMS][V], gc[ITEMS][V];
-  if (a.post_kind != CXG_NORM_NONE) {
-    at.params(a.post_w, 1.f, w1);
-    at.params(a.post_b, 0.f, b1);
-  }
+  // what is the same for all rows, per column: branch_scale * channel gate * (post_w, post_b), pre_w, pre_b
+  const bool post = a.post_kind != CXG_NORM_NONE;
+  float w1[ITEMS][V], b1[ITEMS][V], w2[ITEMS][V], b2[ITEMS][V];
+  at.params(post ? a.post_w : nullptr, 1.f, w1);
+  at.params(post ? a.post_b : nullptr, 0.f, b1);
+  at.params(a.gate_kind == CXG_GATE_CHANNEL ? static_cast<const float*>(a.gate) : nullptr, 1.f, w2);
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float scale = a.branch_scale * w2[i][j];
+      w1[i][j] *= scale;
+      b1[i][j] *= scale;
+    }
   if (a.pre_kind != CXG_NORM_NONE) {
     at.params(a.pre_w, 1.f, w2);
     at.params(a.pre_b, 0.f, b2);
   }
-  if (a.gate_kind == CXG_GATE_CHANNEL) at.params(static_cast<const float*>(a.gate), 1.f, gc);
 
   // every lane stays in the loop as long as its block: the reductions need whole waves
   for (int64_t base = (int64_t)blockIdx.x * kTeams; base < a.rows; base += (int64_t)gridDim.x * kTeams) {
@@ -94,7 +102,7 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a)
     if (a.f) {
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) pf[i].widen(v[i]);
-      if (a.post_kind != CXG_NORM_NONE) {
+      if (post) {
         float s[1];
         if (a.post_kind == CXG_NORM_LAYER) {
           s[0] = 0.f;
@@ -107,12 +115,14 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a)
         }
         s[0] = 0.f;
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
+        for (int i = 0; i < ITEMS; ++i) {
+          const float m = S::TAIL != kRnWhole || at.on[i] ? mean1 : 0.f;     // (columns that do not exist stay 0)
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            v[i][j] -= mean1;
-            s[0] += at.counts(i, j) ? v[i][j] * v[i][j] : 0.f;
+            v[i][j] -= m;
+            s[0] += S::TAIL == kRnWhole || at.counts(i, j) ? v[i][j] * v[i][j] : 0.f;
           }
+        }
         team_sum<S, 1>(s, s_red, slot);
         rstd1 = inverse_sqrt(s[0] * inv_c + a.eps);
 #pragma unroll
@@ -120,7 +130,12 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a)
 #pragma unroll
           for (int j = 0; j < V; ++j) v[i][j] = v[i][j] * rstd1 * w1[i][j] + b1[i][j];
       }
-      const float bs = a.branch_scale * grow;
+      if (!post) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+          for (int j = 0; j < V; ++j) v[i][j] *= w1[i][j];
+      }
       if (a.gate_kind == CXG_GATE_FULL) {
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
@@ -129,18 +144,13 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a)
 #pragma unroll
           for (int j = 0; j < V; ++j) v[i][j] *= g[j];
         }
-      } else if (a.gate_kind == CXG_GATE_CHANNEL) {
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-#pragma unroll
-          for (int j = 0; j < V; ++j) v[i][j] *= gc[i][j];
       }
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) {
         float x[V];
         px[i].widen(x);
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[i][j] = a.res_scale * x[j] + bs * v[i][j];
+        for (int j = 0; j < V; ++j) v[i][j] = a.res_scale * x[j] + grow * v[i][j];
       }
     } else {
 #pragma unroll
@@ -169,12 +179,14 @@ __global__ __launch_bounds__(S::THREADS) void residual_norm_fwd_kernel(RnArgs a)
       }
       s[0] = 0.f;
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i)
+      for (int i = 0; i < ITEMS; ++i) {
+        const float m = S::TAIL != kRnWhole || at.on[i] ? mean2 : 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          v[i][j] -= mean2;
-          s[0] += at.counts(i, j) ? v[i][j] * v[i][j] : 0.f;
+          v[i][j] -= m;
+          s[0] += S::TAIL == kRnWhole || at.counts(i, j) ? v[i][j] * v[i][j] : 0.f;
         }
+      }
       team_sum<S, 1>(s, s_red, slot);
       rstd2 = inverse_sqrt(s[0] * inv_c + a.eps);
       if (live) {
