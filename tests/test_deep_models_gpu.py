@@ -122,6 +122,19 @@ def test_linear_in_bf16_and_with_frozen_weights():
 
 
 @gpu
+def test_typed_linear_checkpoint_refuses_second_derivatives():
+    import cxgnncomp
+    x = torch.randn(90, 64, device="cuda", requires_grad=True)
+    w, types = torch.randn(3, 64, 32, device="cuda", requires_grad=True), torch.randint(0, 3, (90, ), device="cuda")
+    announce("TypedLinearE2EOP checkpoint create_graph")
+    out = cxgnncomp.TypedLinearE2EOP.apply(x, w, types, [], 256, None, "int8")
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        torch.autograd.grad(out.sum(), (x, w), create_graph=True)
+    out = cxgnncomp.TypedLinearE2EOP.apply(x, w, types, [], 256, None, "int8")
+    assert torch.autograd.grad(out.sum(), w)[0].shape == w.shape
+
+
+@gpu
 def test_nothing_is_packed_where_no_backward_pass_follows(monkeypatch):
     """Without gradients (serving) a layer's input is not packed; bad formats are refused all the same."""
     import cxgnncomp

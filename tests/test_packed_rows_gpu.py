@@ -219,6 +219,33 @@ def test_weight_grad_rows_segments_and_maps(m, segs, maps):
 
 
 @gpu
+@pytest.mark.parametrize("k,n", [(60, 30), (100, 3), (100, 50), (300, 40), (300, 2), (300, 70)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_weight_grad_maps_at_every_tile_shape(k, n, dtype):
+    """Row maps with entries outside their matrices, ragged segments and steps, strided rows of g."""
+    import cxgnncomp
+    m = 1500
+    codes, exps, values, g, bounds, src, dst = _wgrad_case(m, k, n, dtype, segs=4, maps=True, seed=k)
+    src[::13] = m
+    dst[5::17] = -1
+    keep = (src < m) & (dst >= 0)
+    wide = torch.zeros(m, n + 5, dtype=dtype)
+    wide[:, 3:n + 3] = g
+    announce("packed_weight_grad maps %d x %d %s" % (k, n, dtype))
+    p = cxgnncomp.PackedRows(codes.cuda(), exps.cuda(), k)
+    gw, gb = cxgnncomp.packed_weight_grad(p, wide.cuda()[:, 3:n + 3], torch.tensor(bounds).cuda(), src_idx=src.cuda(),
+                                          dst_idx=dst.cuda(), want_sums=True)
+    rows = [torch.arange(a, b)[keep[a:b]] for a, b in zip(bounds, bounds[1:])]
+    cuts = [0]
+    for r in rows:
+        cuts.append(cuts[-1] + len(r))
+    order = torch.cat(rows)
+    check(gw, packed_ref.weight_grad(values, g, cuts, src[order], dst[order]), F32, "gw")
+    for r, want in enumerate(packed_ref.row_sums(g, cuts, dst[order])):
+        check(gb[r], want, F32, "sums of segment %d" % r)
+
+
+@gpu
 @pytest.mark.parametrize("m,n", [(0, 5), (1, 3), (33, 1), (700, 47), (5000, 72), (1300, 300)])
 @pytest.mark.parametrize("k", [20, 140])
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])

@@ -370,3 +370,19 @@ def test_module_and_a_changed_input():
         fc.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+@gpu
+@pytest.mark.parametrize("eps", [0.0, 1e-42])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+def test_rows_whose_squares_are_below_the_smallest_normal_number(eps, kind):
+    """Mean squares near 1e-40 keep some 16 bits: the result is within 2^-10 of the formula in 64 bits."""
+    import cxgnncomp
+    x = torch.randn(9, 64, generator=torch.Generator().manual_seed(3)) * 1e-20
+    announce("residual_norm %s of tiny rows, eps %g" % (kind, eps))
+    _, y = cxgnncomp.residual_norm(x.cuda(), None, pre=kind, eps=eps)
+    v = x.double()
+    if kind == "layer":
+        v = v - v.mean(1, keepdim=True)
+    want = v / (v.square().mean(1, keepdim=True) + eps).sqrt()
+    assert ((y.cpu().double() - want).abs() <= 2.0 ** -10 * want.abs() + 2.0 ** -12).all()
