@@ -14,9 +14,9 @@
 // Layout: codes [rows][pitch] with the columns rounded up to 16 (zeros behind the last), one
 // exponent byte k + 127 per group, [rows][groups].
 //
-// Bound: memory, one pass.  Eight lanes own a group (two where a row is that short) and hold its values in registers between
-// the maximum (integer maxima of the magnitudes' bits, so that a NaN is largest; three data-parallel
-// moves) and the rounding; a piece of the group is 128 contiguous bytes over the eight lanes.
+// Bound: memory, one pass.  Eight lanes own a group (two or four where a row is that short) and hold its
+// values in registers between the maximum (integer maxima of the magnitudes' bits, so that a NaN is largest;
+// three data-parallel moves) and the rounding; a piece of the group is 128 contiguous bytes over the eight lanes.
 // Measured: 2,449,029 x 128 fp32 packed in 289 us = 5.4 TB/s (a 4 GiB copy: 4.7 TB/s).
 #include "packed_rows.hpp"
 
@@ -24,10 +24,9 @@ namespace cxg {
 namespace {
 
 constexpr int kPrThreads = 256;
-// Lanes per group, sixteen columns each: eight, or two for rows of at most 32 columns (48 M bf16 values in
-// rows of 16: 28 us against 82 us).
-constexpr int kPrLanes = 8, kPrLanesNarrow = 2;
-inline bool pr_narrow(int cols) { return cols <= 16 * kPrLanesNarrow; }
+// Lanes per group, sixteen columns each: eight, or two / four for rows of at most 32 / 64 columns (48 M bf16
+// values in rows of 16: 28 us against 82 us, of 47: 34 us against 48 us).
+inline int pr_lanes(int cols) { return cols <= 32 ? 2 : cols <= 64 ? 4 : 8; }
 
 struct PackArgs {
   const void* x; int64_t ldx;
@@ -35,6 +34,24 @@ struct PackArgs {
   void* out;
   int64_t rows;
   int cols, pitch, groups;
+};
+
+// Team `team` of a block that starts at group `first` of the matrix, groups counted row by row: the teams of
+// a wave share the lines that groups end in, and a row's last, short group does not cost a block of its own
+// (one row of blocks per group: 48 M bf16 values in rows of 200 36 us, 26 us; of 805 38 + 38 us, 33 + 25).
+struct PackPlace {
+  int64_t row0;                          // row of the block's first group, the same for all lanes
+  int row, group;                        // row after that, group in the row
+  bool live;
+  __device__ __forceinline__ PackPlace(const PackArgs& a, int64_t first, int team) {
+    row0 = a.groups == 1 ? first : first / a.groups;
+    const unsigned n = (unsigned)(first - row0 * a.groups) + (unsigned)team, d = (unsigned)a.groups;
+    // n / d: at most 1 where d > team, and n * (2^16 / d + 1) / 2^16 is exact for d < 32 and n < 2^8
+    row = (int)(d >= 32 ? (n >= d ? 1u : 0u) : (n * (65536u / d + 1u)) >> 16);
+    group = (int)(n - (unsigned)row * d);
+    live = row0 + row < a.rows;
+  }
+  template <typename T> __device__ __forceinline__ T* of(T* p, int64_t ld) const { return p + row0 * ld + row * ld; }
 };
 
 template <int CTRL> __device__ __forceinline__ unsigned moved_max(unsigned m) {
@@ -69,16 +86,17 @@ template <int FMT> __device__ __forceinline__ unsigned encode4(const float* v, f
 
 template <typename T, int FMT, int LANES> __global__ __launch_bounds__(kPrThreads) void pack_rows_kernel(PackArgs a) {
   constexpr int V = 16 / sizeof(T), kPieces = 16 / V, kTeams = kPrThreads / LANES;
-  const int lit = threadIdx.x % LANES, group = blockIdx.y;
-  const int c0 = group * kPrGroup;
-  for (int64_t base = (int64_t)blockIdx.x * kTeams; base < a.rows; base += (int64_t)gridDim.x * kTeams) {
-    const int64_t row = base + threadIdx.x / LANES;
-    const bool live = row < a.rows;                      // dead teams stay: the moves need whole waves
-    const T* const src = static_cast<const T*>(a.x) + (live ? row : 0) * a.ldx;
+  static_assert(kTeams <= 32 || LANES < 8, "PackPlace");             // (narrow rows are one group)
+  const int lit = threadIdx.x % LANES;
+  const int64_t all = a.rows * a.groups;
+  for (int64_t base = (int64_t)blockIdx.x * kTeams; base < all; base += (int64_t)gridDim.x * kTeams) {
+    const PackPlace at(a, base, threadIdx.x / LANES);
+    const int c0 = at.group * kPrGroup, cols = at.live ? a.cols : 0;   // dead teams stay: the moves need whole waves
+    const T* const src = at.of(static_cast<const T*>(a.x), a.ldx);
     float v[kPieces][V];
     RowPiece<T, V> raw[kPieces];
 #pragma unroll
-    for (int p = 0; p < kPieces; ++p) raw[p].load(src, c0 + (p * LANES + lit) * V, a.cols);
+    for (int p = 0; p < kPieces; ++p) raw[p].load(src, c0 + (p * LANES + lit) * V, cols);
     unsigned top = 0;
 #pragma unroll
     for (int p = 0; p < kPieces; ++p) {
@@ -90,18 +108,17 @@ template <typename T, int FMT, int LANES> __global__ __launch_bounds__(kPrThread
       }
     }
     top = moved_max<0xB1>(top);                          // quad_perm [1,0,3,2]
-    if constexpr (LANES == 8) {
-      top = moved_max<0x4E>(top);                        // quad_perm [2,3,0,1]
-      top = moved_max<0x141>(top);                       // row_half_mirror
-    }
+    if constexpr (LANES >= 4) top = moved_max<0x4E>(top);            // quad_perm [2,3,0,1]
+    if constexpr (LANES >= 8) top = moved_max<0x141>(top);           // row_half_mirror
     const int b = exponent_byte<FMT>(top);
     const float inv = __uint_as_float((unsigned)(254 - b) << 23);
-    if (!live) continue;
+    if (!at.live) continue;
+    uint8_t* const out = at.of(a.codes, a.pitch);
 #pragma unroll
     for (int p = 0; p < kPieces; ++p) {
       const int c = c0 + (p * LANES + lit) * V;
       if (c >= a.pitch) continue;
-      uint8_t* const dst = a.codes + row * a.pitch + c;
+      uint8_t* const dst = out + c;
       unsigned w[V / 4];
 #pragma unroll
       for (int q = 0; q < V / 4; ++q) w[q] = b == kPrNotFinite ? 0u : encode4<FMT>(&v[p][4 * q], inv);
@@ -111,34 +128,34 @@ template <typename T, int FMT, int LANES> __global__ __launch_bounds__(kPrThread
         *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
       }
     }
-    if (lit == 0) a.exps[row * a.groups + group] = (uint8_t)b;
+    if (lit == 0) at.of(a.exps, a.groups)[at.group] = (uint8_t)b;
   }
 }
 
 template <typename T, int FMT, int LANES> __global__ __launch_bounds__(kPrThreads) void unpack_rows_kernel(PackArgs a) {
   constexpr int V = 16 / sizeof(T), kPieces = 16 / V, kTeams = kPrThreads / LANES;
-  const int lit = threadIdx.x % LANES, group = blockIdx.y;
-  const int c0 = group * kPrGroup;
-  for (int64_t row = (int64_t)blockIdx.x * kTeams + threadIdx.x / LANES; row < a.rows;
-       row += (int64_t)gridDim.x * kTeams) {
-    const uint8_t* const src = a.codes + row * a.pitch;
-    unsigned w[kPieces][V / 4];
+  const int lit = threadIdx.x % LANES;
+  const int64_t all = a.rows * a.groups;
+  for (int64_t base = (int64_t)blockIdx.x * kTeams; base < all; base += (int64_t)gridDim.x * kTeams) {
+    const PackPlace at(a, base, threadIdx.x / LANES);
+    if (!at.live) continue;
+    const int c0 = at.group * kPrGroup;
+    const uint8_t* const src = at.of<const uint8_t>(a.codes, a.pitch);
+    // the piece that would pass the end of the row is moved back to end there (values of its neighbour, stored
+    // twice) unless its group is shorter: 48 M bf16 values in rows of 47 30 us, value by value 62
+    typedef unsigned words_t __attribute__((ext_vector_type(V / 4)));
+    typedef words_t loose_t __attribute__((aligned(1)));
+    words_t w[kPieces];
+    int col[kPieces];
 #pragma unroll
     for (int p = 0; p < kPieces; ++p) {
-      const int c = c0 + (p * LANES + lit) * V;
-#pragma unroll
-      for (int q = 0; q < V / 4; ++q) w[p][q] = 0;
-      if (c < a.pitch) {
-        if constexpr (V == 4) {
-          w[p][0] = *reinterpret_cast<const unsigned*>(src + c);
-        } else {
-          const uint2 t = *reinterpret_cast<const uint2*>(src + c);
-          w[p][0] = t.x; w[p][1] = t.y;
-        }
-      }
+      col[p] = c0 + (p * LANES + lit) * V;
+      if (col[p] < a.cols && col[p] + V > a.cols && a.cols - V >= c0) col[p] = a.cols - V;
+      w[p] = 0;
+      if (col[p] < a.cols) w[p] = *reinterpret_cast<const loose_t*>(src + col[p]);      // (inside the pitch)
     }
-    const float scale = packed_scale(a.exps[row * a.groups + group]);
-    T* const dst = static_cast<T*>(a.out) + row * a.cols;
+    const float scale = packed_scale(at.of(a.exps, a.groups)[at.group]);
+    T* const dst = at.of(static_cast<T*>(a.out), a.cols);
 #pragma unroll
     for (int p = 0; p < kPieces; ++p) {
       float v[V];
@@ -146,7 +163,7 @@ template <typename T, int FMT, int LANES> __global__ __launch_bounds__(kPrThread
       for (int q = 0; q < V / 4; ++q) decode4<FMT>(w[p][q], scale, &v[4 * q]);
       RowPiece<T, V> o;
       o.narrow(v);
-      o.store(dst, c0 + (p * LANES + lit) * V, a.cols);
+      o.store(dst, col[p], a.cols);
     }
   }
 }
@@ -159,20 +176,19 @@ int pack_check(int type, int fmt, int64_t rows, int cols) {
   return CXG_OK;
 }
 
+// (more groups per block than this fills: a loop)
 dim3 pack_grid(int64_t rows, int groups, int teams) {
-  int64_t x = ceil_div(rows, (int64_t)teams);
-  const int64_t most = groups >= 64 ? 256 : 16384 / groups;      // rows per block beyond that: a loop
-  return dim3((unsigned)(x < most ? x : most), (unsigned)groups);
+  const int64_t x = ceil_div(rows * groups, (int64_t)teams);
+  return dim3((unsigned)(x < 16384 ? x : 16384));
 }
 
 #define CXG_PR_LAUNCH_LANES(KERNEL, T, FMT)                                                                \
   do {                                                                                                     \
-    if (pr_narrow(a.cols))                                                                                 \
-      hipLaunchKernelGGL((KERNEL<T, FMT, kPrLanesNarrow>), pack_grid(rows, 1, kPrThreads / kPrLanesNarrow), \
-                         dim3(kPrThreads), 0, st, a);                                                      \
-    else                                                                                                   \
-      hipLaunchKernelGGL((KERNEL<T, FMT, kPrLanes>), pack_grid(rows, a.groups, kPrThreads / kPrLanes),     \
-                         dim3(kPrThreads), 0, st, a);                                                      \
+    const int lanes = pr_lanes(a.cols);                                                                    \
+    const dim3 grid = pack_grid(rows, a.groups, kPrThreads / lanes), block(kPrThreads);                    \
+    if (lanes == 2) hipLaunchKernelGGL((KERNEL<T, FMT, 2>), grid, block, 0, st, a);                        \
+    else if (lanes == 4) hipLaunchKernelGGL((KERNEL<T, FMT, 4>), grid, block, 0, st, a);                   \
+    else hipLaunchKernelGGL((KERNEL<T, FMT, 8>), grid, block, 0, st, a);                                   \
   } while (0)
 #define CXG_PR_LAUNCH_FMT(KERNEL, T)                                                                       \
   do {                                                                                                     \
