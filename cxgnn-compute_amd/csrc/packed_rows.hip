@@ -10,6 +10,9 @@
 // (packed_wgrad.hip).  int8 keeps 7 bits below the group's largest power of two, e4m3 keeps 3 bits
 // of every value down to 2^-6 * 2^k: the first for even rows, the second for rows of a wide range.
 // A group with an infinity or a NaN has exponent byte 255 and codes 0: it reads back as NaN.
+// A finite value is off by at most half a step of its code (2^(k-1) for int8; 1/16 of itself or 2^(k-10) for
+// e4m3).  In fp16 the codes' 65536 reads back as 65504, so that finite fp16 rows stay finite; a value that rounds up
+// to 2^128 has no finite fp32 or bf16 form and reads back as an infinity.
 //
 // Layout: codes [rows][pitch] with the columns rounded up to 16 (zeros behind the last), one
 // exponent byte k + 127 per group, [rows][groups].
@@ -18,6 +21,8 @@
 // values in registers between the maximum (integer maxima of the magnitudes' bits, so that a NaN is largest;
 // three data-parallel moves) and the rounding; a piece of the group is 128 contiguous bytes over the eight lanes.
 // Measured: 2,449,029 x 128 fp32 packed in 289 us = 5.4 TB/s (a 4 GiB copy: 4.7 TB/s).
+#include <type_traits>
+
 #include "packed_rows.hpp"
 
 namespace cxg {
@@ -161,6 +166,14 @@ template <typename T, int FMT, int LANES> __global__ __launch_bounds__(kPrThread
       float v[V];
 #pragma unroll
       for (int q = 0; q < V / 4; ++q) decode4<FMT>(w[p][q], scale, &v[4 * q]);
+      if constexpr (std::is_same<T, f16_t>::value) {
+        // fp16 values next to the largest, 65504, are held as 65536 and stay finite.  (448 * 2^7 and 127 * 2^9 are
+        // below that: only groups of a large scale are looked through.)
+        if (scale >= 256.f) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) v[j] = __builtin_fabsf(v[j]) == 65536.f ? __builtin_copysignf(65504.f, v[j]) : v[j];
+        }
+      }
       RowPiece<T, V> o;
       o.narrow(v);
       o.store(dst, col[p], a.cols);

@@ -46,7 +46,9 @@ class PackedRows:
         return self.codes.numel() + self.exps.numel()
 
     def unpack(self, dtype=None):
-        """The rows [N, cols] in ``dtype`` (the one they had): exact in float32 and bfloat16."""
+        """The rows [N, cols] in ``dtype`` (the one they had): exact in float32 and bfloat16.  In float16 a magnitude
+        of 65536, as which values next to the largest float16 are held, reads back as 65504: finite float16
+        rows stay finite.  Larger ones (of rows that had a wider dtype) become infinities."""
         return _ops._C.unpack_rows(self.codes, self.exps, self.cols, FORMATS[self.fmt], dtype or self.dtype)
 
     def __repr__(self):
@@ -57,9 +59,9 @@ def pack_rows(x, fmt="int8"):
     """x [N, C] (CUDA, float32 / bfloat16 / float16, rows may be strided) in 8 bits per value and one
     byte per 128 columns.  Codes are x / 2^k rounded to the nearest, ties to even, 2^k the smallest power
     of two (2^-111 at least) with which the group's largest magnitude stays within 127 ("int8") or
-    448 ("e4m3"): an int8 value is off by at most 1/127 of the group's largest magnitude, an e4m3 value
-    by at most 1/16 of itself or 2^-10 * 2^k (a value that rounds up to 2^128 reads back as an infinity, as it
-    would from bfloat16).  Not differentiable; packing unpacked rows gives the same codes."""
+    448 ("e4m3"): an int8 value is off by at most 2^(k-1), which is 1/127 of the group's largest magnitude or less
+    (k > -111), an e4m3 value by at most 1/16 of itself or 2^(k-10) (a value that rounds up to 2^128 reads back
+    as an infinity).  Not differentiable; packing unpacked rows gives the same codes."""
     codes, exps = _ops._C.pack_rows(x, _format(fmt))
     return PackedRows(codes, exps, x.shape[1], fmt, x.dtype)
 

@@ -799,8 +799,9 @@ int cxg_residual_norm_bwd(const void* x, int64_t ldx, const void* f, int64_t ldf
  * ties to even; b is the smallest byte (at least 16) with which the largest magnitude fits: 127 after
  * rounding (int8) or 448 (e4m3).  A group with an infinity or NaN has b = 255, codes 0, and reads back
  * as NaN.  codes is [rows][cxg_packed_pitch(cols)] (columns rounded up to 16, zeros behind the last;
- * 16-byte aligned), exps [rows][cxg_packed_groups(cols)].  Unpacking is exact in fp32 and bf16 (in
- * fp16 it rounds) and writes contiguous rows.
+ * 16-byte aligned), exps [rows][cxg_packed_groups(cols)].  Unpacking writes contiguous rows and is exact in
+ * fp32 and bf16; in fp16 it rounds, and a magnitude of 65536 (as which values next to the largest fp16 are
+ * held) becomes 65504.
  */
 int cxg_packed_pitch(int cols);
 int cxg_packed_groups(int cols);

@@ -1,0 +1,75 @@
+"""Calls of the row operators (residual norm, rows in 8 bits, their weight gradient, linear maps and layers on
+them) that the documentation allows or refuses, beside the shapes of the other files."""
+import pytest
+import torch
+
+import packed_ref
+from conftest import announce
+
+gpu = pytest.mark.gpu
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def _half_step(values, exps, cols, fmt):
+    """What a value may be off by: half a step of its code."""
+    scale = packed_ref.spread(exps, cols)
+    if fmt == "int8":
+        return scale / 2
+    return torch.maximum(values.abs() / 16, scale * 2.0 ** -10)
+
+
+def _large_fp16_rows():
+    x = torch.zeros(12, 200, dtype=F16)
+    large = torch.tensor([65504.0, 65472.0, 65280.0, 65248.0, 65056.0, 65024.0, 64992.0, 63488.0, 63456.0, 61440.0, 40000.0, 1.0], dtype=F16)
+    for r in range(12):
+        x[r, : 12 - r] = large[r:]                       # every one of them is some row's largest
+        x[r, 100:112 - r] = -large[r:]
+        x[r, 128 + r:140] = large[r:]
+    return x
+
+
+# ----------------------------------------- on the CPU ------------------------------------------- #
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_large_fp16_values_are_held_within_half_a_step(fmt):
+    """The 8-bit form of finite fp16 rows is at most 65536 and off by half a step; 65504 in its place is too."""
+    x = _large_fp16_rows()
+    _, exps, values = packed_ref.pack(x, fmt)
+    assert float(values.abs().max()) == 65536.0
+    for v in (values, values.clamp(-65504.0, 65504.0)):
+        assert ((v - x.double()).abs() <= _half_step(x.double(), exps, 200, fmt)).all()
+
+
+# ------------------------------------------ on the GPU ------------------------------------------- #
+@gpu
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_finite_fp16_rows_read_back_finite(fmt):
+    import cxgnncomp
+    x = _large_fp16_rows()
+    announce("unpack large fp16 rows %s" % fmt)
+    for cols in (200, 190, 45, 12):                      # whole and moved-back pieces, every number of lanes
+        p = cxgnncomp.pack_rows(x[:, :cols].contiguous().cuda(), fmt)
+        codes, exps, values = packed_ref.pack(x[:, :cols], fmt)
+        assert torch.equal(p.codes.cpu(), codes) and torch.equal(p.exps.cpu(), exps)
+        back = p.unpack()
+        assert back.dtype == F16 and torch.equal(back.cpu(), values.clamp(-65504.0, 65504.0).half())
+        again = cxgnncomp.pack_rows(back, fmt)           # packing what was unpacked gives the same codes
+        assert torch.equal(again.codes, p.codes) and torch.equal(again.exps, p.exps)
+        assert torch.equal(p.unpack(F32).cpu().double(), values) and torch.equal(p.unpack(BF16).cpu().double(), values)
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_wider_rows_unpacked_to_fp16_overflow_as_a_cast_does(fmt):
+    import cxgnncomp
+    x = torch.zeros(4, 130)
+    x[0, :3] = torch.tensor([1e5, -1e5, 3.0])
+    x[1, :2] = torch.tensor([65000.0, -66000.0])
+    x[2, 7] = float("nan")
+    x[3, 129] = 1e30
+    announce("unpack fp32 rows to fp16 %s" % fmt)
+    p = cxgnncomp.pack_rows(x.cuda(), fmt)
+    _, _, values = packed_ref.pack(x, fmt)
+    want = torch.where(values.abs() == 65536, values.sign() * 65504, values).half()
+    got = p.unpack(F16).cpu()
+    assert torch.isinf(got[0, 0]) and torch.isinf(got[3, 129]) and torch.isnan(got[2, :128]).all()
+    assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(want)) and torch.equal(torch.isnan(got), torch.isnan(want))
