@@ -1140,6 +1140,8 @@ std::tuple<OptTensor, OptTensor> residual_norm(const Tensor& x, const OptTensor&
     if (given[i].has_value() && given[i]->defined()) {
       c.t[i] = *given[i];
       grad = grad || c.t[i].requires_grad();
+      // (the outputs below would carry no tangent, which reads as a derivative of zero)
+      if (c.t[i]._fw_grad(0).defined()) throw std::runtime_error("residual_norm has no forward-mode derivatives");
     }
   OptTensor r, y;
   if (grad && at::GradMode::is_enabled()) {

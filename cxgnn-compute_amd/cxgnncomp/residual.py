@@ -30,7 +30,7 @@ def residual_norm(x, f, gate=None, *, post=None, post_weight=None, post_bias=Non
 
     One autograd node (csrc_ext/backend_ext.cpp): its backward pass reads x, f, the gate and two
     statistics per norm and row; r and y are not kept.  Gradients of every tensor argument, once (no
-    second derivatives); the sums over rows behind the
+    second and no forward-mode derivatives: both raise); the sums over rows behind the
     vectors' gradients are added in a fixed order, so they repeat bit for bit.
     """
     r, y = _residual_norm(x, f, gate, post, post_weight, post_bias, pre, pre_weight, pre_bias, res_scale, branch_scale, eps)

@@ -73,3 +73,26 @@ def test_wider_rows_unpacked_to_fp16_overflow_as_a_cast_does(fmt):
     got = p.unpack(F16).cpu()
     assert torch.isinf(got[0, 0]) and torch.isinf(got[3, 129]) and torch.isnan(got[2, :128]).all()
     assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(want)) and torch.equal(torch.isnan(got), torch.isnan(want))
+
+
+@gpu
+@pytest.mark.parametrize("which", ["x", "f", "gate", "pre_weight"])
+@pytest.mark.parametrize("mode", ["no_grad", "grad", "leaf"])
+def test_residual_norm_refuses_forward_mode_derivatives(which, mode):
+    """An argument with a tangent is refused, whether or not others take part in a backward pass."""
+    import cxgnncomp
+    from torch.autograd import forward_ad
+    t = {"x": torch.randn(5, 8, device="cuda"), "f": torch.randn(5, 8, device="cuda"), "gate": torch.ones(8, device="cuda"),
+         "pre_weight": torch.ones(8, device="cuda")}
+    if mode == "leaf":
+        t["f" if which == "x" else "x"].requires_grad_(True)
+    announce("residual_norm of a dual tensor %s %s" % (which, mode))
+    with forward_ad.dual_level():
+        t[which] = forward_ad.make_dual(t[which].detach(), torch.ones_like(t[which]))
+        with torch.set_grad_enabled(mode != "no_grad"):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                cxgnncomp.residual_norm(t["x"], t["f"], t["gate"], pre_weight=t["pre_weight"])
+            if which in ("x", "pre_weight"):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    cxgnncomp.residual_norm(t["x"], None, pre_weight=t["pre_weight"])
+    cxgnncomp.residual_norm(t["x"], t["f"], t["gate"], pre_weight=t["pre_weight"])      # outside the level: no tangents
