@@ -440,7 +440,14 @@ template <typename F> auto pw_shaped(int K, int N, F run) {
 // that is not full then costs little).  The tiles of a chunk run on one die: a round is full with as many
 // chunks as fit on each die whole, the same number everywhere, the ragged last chunks of the segments among
 // them (30,289 x 529 x 505 of 3 types, 12 tiles, in bf16: 42 chunks, six on two of the dies, 108 us; 40
-// chunks, five on each, 76 us).
+// chunks, five on each, 76 us).  Ragged chunks have a place as long as they take at most half of it.  With more
+// segments than that most chunks are short, they come on top, and a long segment is still split over the chip
+// (1 M x 512 x 512 of 200 types, half of the rows in one, in fp32: 7.8 ms; with the place taken by ragged
+// chunks a chunk was all rows and the long segment ran on eight blocks, 37.7 ms).  A chunk has at most kPwMaxChunk
+// rows, whatever the width of gW: as many products, times the parts of G, are the longest sum in one fp32
+// accumulator.  (At half as many rows 2 M x 1,024 x 1,024 in bf16 takes 5.3 ms for 5.0, partial tiles.)
+constexpr int64_t kPwMaxChunk = 65536;
+
 int64_t pw_tiles(int K, int N) {
   return pw_shaped(K, N, [&](auto s) { return ceil_div(K, s.KT) * ceil_div(N, s.NT); });
 }
@@ -450,12 +457,13 @@ int64_t pw_chunk_rows(int64_t M, int K, int N, int R) {
   const int64_t slots = 256 / kPwXcds * pw_shaped(K, N, [](auto s) { return (int64_t)s.BLOCKS; });   // of one die
   auto fill = [&](int64_t rounds) {                       // rows so that about `rounds` rounds are full
     const int64_t each = slots * rounds / tiles;          // chunks per die
-    const int64_t chunks = kPwXcds * (each < 1 ? 1 : each) - (R - 1);
-    return ceil_div(M, chunks < 1 ? 1 : chunks);
+    const int64_t place = kPwXcds * (each < 1 ? 1 : each), ragged = R - 1;
+    return ceil_div(M, ragged <= place / 2 ? place - ragged : place);
   };
   const int64_t longest = fill(1), shortest = fill(2);
   int64_t rows = 2048;
   rows = rows > longest ? longest : rows < shortest ? shortest : rows;
+  if (rows > kPwMaxChunk) rows = ceil_div(M, kPwXcds * ceil_div(M, kPwXcds * kPwMaxChunk));   // as many on each die
   return rows < 1 ? 64 : ceil_div(rows, (int64_t)64) * 64;
 }
 

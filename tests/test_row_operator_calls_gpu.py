@@ -39,6 +39,26 @@ def test_large_fp16_values_are_held_within_half_a_step(fmt):
         assert ((v - x.double()).abs() <= _half_step(x.double(), exps, 200, fmt)).all()
 
 
+def _chunks(m, k, n, segs):
+    """Row chunks for which the weight gradient takes workspace."""
+    from cxgnncomp_backend import _lib
+    return (_lib.load().cxg_packed_wgrad_workspace_bytes(m, k, n, segs) - 256) // (4 * n * (k + 1))
+
+
+@pytest.mark.parametrize("k,n", [(64, 64), (128, 128), (512, 512), (600, 600), (1024, 1024), (2048, 2048), (4096, 4096)])
+def test_rows_per_chunk_with_any_number_of_segments(k, n):
+    """What is left of the chunks when every segment but one ends in a ragged one splits a segment of nearly all rows
+    at least as finely as one segment is split at most half as finely; no chunk is longer than 65,536 rows."""
+    for m in (20000, 400000, 2332486):
+        whole = _chunks(m, k, n, 1)
+        assert whole * 65536 >= m
+        for segs in (2, 7, 33, 40, 65, 129, 200, 237, 1000, 5000):
+            left = _chunks(m, k, n, segs) - (segs - 1)
+            # (chunks of at least 64 rows; counts are rounded up to a multiple of eight)
+            assert left >= min(whole // 2, m // 64) - 8 and left * 65536 >= m, (m, segs, left, whole)
+            assert _chunks(m, k, n, segs) <= 2 * whole + segs + 8, (m, segs)
+
+
 # ------------------------------------------ on the GPU ------------------------------------------- #
 @gpu
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
@@ -96,3 +116,37 @@ def test_residual_norm_refuses_forward_mode_derivatives(which, mode):
                 with pytest.raises(RuntimeError, match="forward-mode"):
                     cxgnncomp.residual_norm(t["x"], None, pre_weight=t["pre_weight"])
     cxgnncomp.residual_norm(t["x"], t["f"], t["gate"], pre_weight=t["pre_weight"])      # outside the level: no tangents
+
+
+@gpu
+@pytest.mark.parametrize("m,k,n,segs,share", [(100000, 1024, 1024, 40, 0.9), (60000, 512, 512, 200, 0.5), (50000, 300, 200, 700, 0.7), (20000, 64, 40, 3000, 0.3),
+                                              (300000, 2048, 2048, 1, 1.0), (400000, 1024, 1024, 1, 1.0)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_weight_grad_of_many_segments_and_of_long_chunks(m, k, n, segs, share, dtype):
+    """Skewed segments, more of them than chunks fit the chip at once, and the longest chunks: every segment's 2-norm of
+    the error stays where fp32 accumulation of a chunk puts it (random roundings: 2^-24 * sqrt(products of a chunk) of
+    the result); the sums of G's rows too; results repeat bit for bit."""
+    import cxgnncomp
+    torch.manual_seed(0)
+    big = int(m * share)
+    cuts = [0, big] + (torch.sort(torch.randint(big, m + 1, (segs - 2, )))[0].tolist() + [m] if segs > 1 else [])
+    x, g = torch.randn(m, k, device="cuda"), torch.randn(m, n, device="cuda").to(dtype)
+    seg = torch.tensor(cuts, device="cuda")
+    assert seg.shape[0] == segs + 1
+    announce("packed_weight_grad %d x %d x %d, %d segments %s" % (m, k, n, segs, dtype))
+    p = cxgnncomp.pack_rows(x)
+    gw, gb = cxgnncomp.packed_weight_grad(p, g, seg, want_sums=True)
+    again = cxgnncomp.packed_weight_grad(p, g, seg, want_sums=True)
+    assert torch.equal(gw, again[0]) and torch.equal(gb, again[1])
+    chunk = min(65536, -(-m // (_chunks(m, k, n, segs) - (segs - 1) - 7)))      # rows at most (the count is a multiple of eight)
+    bound = 2.0 ** -24 * (chunk * (3 if dtype == F32 else 1)) ** 0.5
+    a = p.unpack().double()
+    for r in [0] + list(range(1, segs, max(1, segs // 30))):
+        b, e = cuts[r], cuts[r + 1]
+        want, sums = a[b:e].t() @ g[b:e].double(), g[b:e].double().sum(0)
+        if b == e:
+            assert not gw[r].any() and not gb[r].any()
+            continue
+        # (a short segment: one rounding at least)
+        assert float((gw[r] - want).norm()) <= max(bound, 2.0 ** -22) * float(want.norm()), r
+        assert float((gb[r] - sums).norm()) <= max(bound, 2.0 ** -22) * float(sums.norm()), r
