@@ -40,6 +40,7 @@ typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 
 constexpr int kPwThreads = 256;
 constexpr int kPwXcds = 8;               // accelerator dies, one L2 each
+constexpr int64_t kPwMaxBlocks = ((int64_t)1 << 32) / kPwThreads;     // a launch has fewer than 2^32 threads
 constexpr int kPwFront = 8;              // columns in front of a tile of G: at least what a thread stages
 
 // Shape of a block: KT columns of A, NT of G, ROWS rows per step, BLOCKS of them per CU.
@@ -586,18 +587,19 @@ int cxg_packed_wgrad(const uint8_t* codes, const uint8_t* exps, int fmt, int64_t
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const int64_t chunks = pw_chunk_count(M, K, N, R);
   const int64_t tiles = pw_tiles(K, N);
-  CXG_REQUIRE(chunks * tiles < ((int64_t)1 << 31), CXG_ERR_UNSUPPORTED, "too many tiles for one launch");
   const PwArgs a{codes, exps, a_rows, g, ldg, g_rows, src_idx, dst_idx, seg_ptr, M, K, N, R, packed_pitch(K), packed_groups(K),
                  pw_chunk_rows(M, K, N, R), chunks, static_cast<float*>(workspace), (int64_t)K * N + (gb ? N : 0)};
+  // many chunks per segment: sixteen runs of them, else four; four elements at a time where the shapes allow
+  const bool many = chunks > 64 * (int64_t)R;
+  const bool vec = (int64_t)K * N % 4 == 0 && (!gb || N % 4 == 0) && (((uintptr_t)gw | (uintptr_t)gb) & 15) == 0;
+  const int64_t sums = ceil_div(a.stride, (int64_t)(vec ? 4 : 1) * (many ? 16 : 64));           // blocks per segment
+  CXG_REQUIRE(chunks * tiles < kPwMaxBlocks && sums < kPwMaxBlocks, CXG_ERR_UNSUPPORTED, "gw of %d x %d is too large for one launch",
+              K, N);
   if (M > 0) {
     if (fmt == CXG_PACK_INT8) pw_launch_type<CXG_PACK_INT8>(a, g_type, chunks, st);
     else pw_launch_type<CXG_PACK_E4M3>(a, g_type, chunks, st);
     CXG_LAUNCH_CHECK("packed_wgrad_kernel");
   }
-  CXG_REQUIRE(a.stride < ((int64_t)1 << 34), CXG_ERR_UNSUPPORTED, "gw too large for one launch");
-  // many chunks per segment: sixteen runs of them, else four; four elements at a time where the shapes allow
-  const bool many = chunks > 64 * (int64_t)R;
-  const bool vec = (int64_t)K * N % 4 == 0 && (!gb || N % 4 == 0) && (((uintptr_t)gw | (uintptr_t)gb) & 15) == 0;
   if (vec && many) pw_launch_sums<4, 16>(a, gw, gb, st);
   else if (vec) pw_launch_sums<4, 4>(a, gw, gb, st);
   else if (many) pw_launch_sums<1, 16>(a, gw, gb, st);

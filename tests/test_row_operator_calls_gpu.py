@@ -59,6 +59,16 @@ def test_rows_per_chunk_with_any_number_of_segments(k, n):
             assert _chunks(m, k, n, segs) <= 2 * whole + segs + 8, (m, segs)
 
 
+def test_a_weight_gradient_too_large_for_a_launch_is_refused_before_any():
+    """(Status -2, not the -4 of a launch that failed; all of it on the host.)"""
+    from cxgnncomp_backend import _lib
+    lib = _lib.load()
+    for k, n, segs in ((1 << 17, 1 << 17, 1), (1 << 22, 1 << 22, 1), (1 << 18, (1 << 16) + 1, 3)):
+        need = lib.cxg_packed_wgrad_workspace_bytes(10, k, n, segs)
+        assert lib.cxg_packed_wgrad(256, 256, 0, 10, 256, n, 0, 10, None, None, 256, 10, k, n, segs, 256, None, 256, need, None) == -2
+        assert b"too large" in lib.cxg_last_error()
+
+
 # ------------------------------------------ on the GPU ------------------------------------------- #
 @gpu
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
