@@ -339,9 +339,17 @@ def _weight_grad(x, g):
     """g^T x, the weight gradient of ``F.linear(x, w)``: one very long reduction axis, on the
     typed weight-gradient kernel as a single segment."""
     x2, g2 = x.reshape(-1, x.shape[-1]).contiguous(), g.reshape(-1, g.shape[-1]).contiguous()
+    if g2.dtype != torch.float32:
+        x2 = x2.to(g2.dtype)                                     # (autocast: the output is narrower than the input)
     m = x2.shape[0]
-    full = _typed.typed_gemm_wgrad(x2, g2, _one_segment(m, x.device), m, 1) if m > 0 else None
-    return full[0].t() if full is not None else g2.t() @ x2      # shapes that kernel does not take
+    full = _typed.typed_gemm_wgrad(x2, g2, _one_segment(m, x.device), m, 1) if m > 0 and g2.dtype == torch.float32 else None
+    return full[0].t() if full is not None else g2.t() @ x2      # shapes and types that kernel does not take
+
+
+def _bias_grad(g):
+    """The sum of the rows of g, in fp32 (in 64 bits for float64 rows)."""
+    g = g.reshape(-1, g.shape[-1])
+    return g.sum(dim=0) if g.dtype == torch.float64 else _ops.column_sum(g.float().contiguous())
 
 
 def _mm(x, w_kn, bias=None, addend=None):
@@ -451,11 +459,11 @@ class LinearOP(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             gx = _typed.dense_linear(g, weight) if g.dim() == 2 else None
             if gx is None:
-                gx = g @ weight
+                gx = g @ weight.to(g.dtype)
         if ctx.needs_input_grad[1]:
             gw = _weight_grad(x, g)
         if ctx.needs_input_grad[2]:
-            gb = _ops.column_sum(g.reshape(-1, g.shape[-1]).contiguous())
+            gb = _bias_grad(g)                   # (autograd rounds to the parameters' types)
         grads = (gx, gw, gb, g)              # bias and addend are optional arguments of apply()
         return tuple(grads[i] if need else None for i, need in enumerate(ctx.needs_input_grad))
 
@@ -503,7 +511,7 @@ def _linear_product(x, weight, bias, addend):
 
 def linear(x, weight, bias=None, addend=None, checkpoint=None):
     """``F.linear(x, weight, bias)``, plus ``addend`` where given, for the conv layers; CUDA
-    tensors take LinearOP.  ``checkpoint`` "int8" or "e4m3": what the weight gradient needs of x is
+    tensors take LinearOP (types other than float32 its library products).  ``checkpoint`` "int8" or "e4m3": what the weight gradient needs of x is
     kept in 8 bits per value (PackedLinearOP; CUDA tensors, float32 / bfloat16 / float16)."""
     if check_format(checkpoint) is not None and x.is_cuda and torch.is_grad_enabled():     # else nothing is kept
         if addend is not None and x.dim() != 2:

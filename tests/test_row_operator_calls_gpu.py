@@ -5,6 +5,7 @@ import torch
 
 import packed_ref
 from conftest import announce
+from rounding import B, U, check
 
 gpu = pytest.mark.gpu
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
@@ -160,3 +161,81 @@ def test_weight_grad_of_many_segments_and_of_long_chunks(m, k, n, segs, share, d
         # (a short segment: one rounding at least)
         assert float((gw[r] - want).norm()) <= max(bound, 2.0 ** -22) * float(want.norm()), r
         assert float((gb[r] - sums).norm()) <= max(bound, 2.0 ** -22) * float(sums.norm()), r
+
+
+def _product(a, b, dtype):
+    """a @ b by a library product of ``dtype`` operands: fp32 sums, rounded once to ``dtype``."""
+    a, b = a.to(dtype).double(), b.to(dtype).double()
+    v, mag = a @ b, a.abs() @ b.abs()
+    return B(v, 2 * U * a.shape[1] * mag + torch.finfo(dtype).eps / 2 * (v.abs() + 2 * U * a.shape[1] * mag))
+
+
+@gpu
+@pytest.mark.parametrize("m,k,n", [(300, 90, 33), (5000, 128, 64), (5000, 90, 64), (1, 16, 8)])
+@pytest.mark.parametrize("how", ["bf16", "fp16", "autocast", "bf16 addend", "fp64"])
+def test_linear_without_checkpoint_in_other_types(m, k, n, how):
+    """Forward and backward where neither the split product nor the weight-gradient kernel takes the types."""
+    import cxgnncomp
+    torch.manual_seed(k)
+    dtype = {"bf16": BF16, "fp16": F16, "autocast": BF16, "bf16 addend": BF16, "fp64": torch.float64}[how]
+    held = F32 if how == "autocast" else dtype
+    x, w, b = (torch.randn(s).to(held) for s in ((m, k), (n, k), (n, )))
+    w = w / 8
+    g = torch.randn(m, n).to(dtype)
+    t = [v.cuda().requires_grad_(True) for v in ((x, w, b) + ((torch.randn(m, n).to(held), ) if "addend" in how else ()))]
+    announce("linear %d x %d x %d %s" % (m, k, n, how))
+    with torch.autocast("cuda", dtype=BF16, enabled=how == "autocast"):
+        out = cxgnncomp.linear(*t)
+    if how == "autocast" and out.dtype == F32:           # fp32 inputs that the split product takes stay fp32
+        g, dtype = g.float(), F32
+    grads = torch.autograd.grad(out, t, g.cuda())
+    if how == "fp64":
+        for got, want in zip(grads, (g @ w, g.t() @ x, g.sum(0))):
+            assert got.dtype == dtype and torch.allclose(got.cpu(), want, rtol=1e-12, atol=1e-12)
+        return
+    if dtype == F32:
+        assert (m, k, n) == (5000, 128, 64)
+        for got, want in zip(grads, (g.double() @ w.double(), g.double().t() @ x.double(), g.double().sum(0))):
+            assert float((got.cpu() - want).norm() / want.norm()) < 2.0 ** -20
+        return
+    check(grads[0], _product(g, w, dtype), held, "gx")
+    check(grads[1], _product(g.t(), x, dtype), held, "gw")
+    sums = g.double()
+    check(grads[2], B(sums.sum(0), U * m * 1.01 * sums.abs().sum(0)), held, "gb")
+    if "addend" in how:
+        assert torch.equal(grads[3].cpu(), g)
+
+
+@gpu
+@pytest.mark.parametrize("m,k,n", [(5000, 128, 64), (5000, 90, 64), (300, 90, 33)])
+def test_linear_that_keeps_8_bits_under_autocast(m, k, n):
+    """Output and its type as without checkpoint, on the split product and on the library's; gradients of both."""
+    import cxgnncomp
+    torch.manual_seed(n)
+    x, w, b = (torch.randn(s, device="cuda").requires_grad_(True) for s in ((m, k), (n, k), (n, )))
+    announce("linear checkpoint autocast %d x %d x %d" % (m, k, n))
+    with torch.autocast("cuda", dtype=BF16):
+        out, plain = (cxgnncomp.linear(x, w, b, checkpoint=c) for c in ("int8", None))
+    assert out.dtype == plain.dtype and torch.equal(out, plain)
+    g = torch.randn(m, n, device="cuda").to(out.dtype)
+    got, want = (torch.autograd.grad(o, (x, w, b), g) for o in (out, plain))
+    assert torch.equal(got[0], want[0]) and all(v.dtype == F32 for v in got)
+    weight = packed_ref.weight_grad(packed_ref.pack(x.detach().cpu(), "int8")[2], g.cpu(), [0, m])
+    weight.v, weight.e = weight.v[0].t(), weight.e[0].t()
+    check(got[1], weight, F32, "weight gradient")
+    check(got[2], packed_ref.row_sums(g.cpu(), [0, m])[0], F32, "bias gradient")
+
+
+@gpu
+@pytest.mark.parametrize("m", [300, 5000])
+def test_linear_maps_refuse_forward_mode_derivatives(m):
+    import cxgnncomp
+    from torch.autograd import forward_ad
+    x, w = torch.randn(m, 128, device="cuda"), torch.randn(64, 128, device="cuda")
+    announce("linear of a dual tensor")
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        for checkpoint in (None, "int8"):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError):
+                    cxgnncomp.linear(d, w, checkpoint=checkpoint)
