@@ -209,7 +209,7 @@ class MySageConv(torch.nn.Module):
             out = linear(sage_mean_forward(x, ptr, idx, num_node), self.lin_l.weight, self.lin_l.bias,
                          checkpoint=self.checkpoint)
         if self.root_weight:
-            out = linear(x[:num_node] if num_node != 0 else x, self.lin_r.weight, addend=out, checkpoint=self.checkpoint)
+            out = linear(x[:out.shape[0]], self.lin_r.weight, addend=out, checkpoint=self.checkpoint)
         return out
 
 

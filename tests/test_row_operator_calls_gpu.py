@@ -239,3 +239,30 @@ def test_linear_maps_refuse_forward_mode_derivatives(m):
             for grad in (True, False):
                 with torch.set_grad_enabled(grad), pytest.raises(RuntimeError):
                     cxgnncomp.linear(d, w, checkpoint=checkpoint)
+
+
+@gpu
+@pytest.mark.parametrize("widths", [(16, 24), (24, 16)])
+@pytest.mark.parametrize("num_node", [0, 40])
+def test_sage_layer_with_8_bits_takes_the_rows_it_takes_without(widths, num_node):
+    """More source rows than rows of the graph, all rows asked for as 0, a column slice as input."""
+    import cxgnncomp
+    from cxgnncomp import synthetic as S
+    cxgnncomp.set_timers()
+    ptr, idx = S.uniform_graph(60, 300, seed=0)
+    ptr, idx = ptr.cuda(), idx.cuda()
+    torch.manual_seed(0)
+    conv = cxgnncomp.MySageConv(*widths).cuda()
+    packed = cxgnncomp.MySageConv(*widths, checkpoint="int8").cuda()
+    packed.load_state_dict(conv.state_dict())
+    wide = torch.randn(75, widths[0] + 5, device="cuda")
+    res = []
+    announce("MySageConv %s num_node %d" % (widths, num_node))
+    for layer in (conv, packed):
+        x = wide[:, 2:widths[0] + 2].detach().requires_grad_(True)
+        out = layer(x, ptr, idx, num_node)
+        res.append((out, torch.autograd.grad(out.square().sum(), x)[0]))
+    assert tuple(res[1][0].shape) == (num_node or 60, widths[1])
+    for a, b in zip(*res):
+        # the same products of at most 24 values and means of about five rows, in another order
+        assert float((a - b).detach().abs().max()) <= 2.0 ** -18 * float(a.detach().abs().max())
