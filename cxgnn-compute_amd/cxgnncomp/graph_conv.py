@@ -181,6 +181,8 @@ def run_rgcn4(x, ptr, idx, edge_types, linear, num_center, num_edge, preproccess
 
 class MySageConv(torch.nn.Module):
 
+    checkpoint = None                 # (modules saved before there was one)
+
     def __init__(self, in_channels, hidden_channels, root_weight=True, bias=True, checkpoint=None):
         """``checkpoint`` (not upstream) "int8" or "e4m3": the inputs of the layer's linear maps are kept
         for the backward pass in 8 bits per value (``linear``)."""
@@ -214,6 +216,8 @@ class MySageConv(torch.nn.Module):
 
 
 class MyGINConv(torch.nn.Module):
+
+    checkpoint = None                 # (modules saved before there was one)
 
     def __init__(self, in_channels, hidden_channels, checkpoint=None):
         """``checkpoint`` (not upstream) "int8" or "e4m3": the input of the layer's linear map is kept for
@@ -847,6 +851,8 @@ class MyGATConv(torch.nn.Module):
 
 
 class MyGCNConv(torch.nn.Module):
+
+    checkpoint = None                 # (modules saved before there was one)
 
     def __init__(self, in_channels, out_channels, normalize=False, bias=True, checkpoint=None):
         """``checkpoint`` (not upstream) "int8" or "e4m3": the input of the layer's linear map is kept for

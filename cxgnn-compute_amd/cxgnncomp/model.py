@@ -37,6 +37,7 @@ def _need_csr(graph_type):
 class GNN(torch.nn.Module):
 
     packs_inputs = False              # whether the layers take ``checkpoint``
+    residual = checkpoint = None      # (models saved before there were these options)
 
     def __init__(self, in_channels, hidden_channels, out_channels, num_layer, dropout, graph_type,
                  config=None, residual=None, checkpoint=None, **kwargs):

@@ -1,0 +1,33 @@
+"""Models and layers beside the options that deep stacks have: modules saved before there were any, configurations and
+model classes that do not know them, and what their refusals say.  On the CPU."""
+import copy
+import types
+
+import pytest
+import torch
+
+import cxgnncomp
+
+
+def _as_saved_before(module):
+    """The module as one restored from a file that was written before it had the options."""
+    old = copy.deepcopy(module)
+    for m in old.modules():
+        for name in ("checkpoint", "residual"):
+            m.__dict__.pop(name, None)
+    return old
+
+
+@pytest.mark.parametrize("kind", ["SAGE", "GCN", "GIN", "GAT", "RGCN"])
+def test_modules_saved_before_the_options(kind, monkeypatch):
+    more = {"GAT": dict(heads=1), "RGCN": dict(num_rel=2)}.get(kind, {})
+    model = _as_saved_before(getattr(cxgnncomp, kind)(4, 8, 3, 2, 0.0, "CSR_Layer", **more))
+    assert model.residual is None and model.checkpoint is None
+    model.reset_parameters()
+    if kind in ("SAGE", "GCN", "GIN"):
+        assert all(conv.checkpoint is None for conv in model.convs)
+    # the forward pass up to the layers, which need a GPU
+    monkeypatch.setattr(type(model), "layer", lambda self, conv, x, batch, i: x @ torch.ones(x.shape[1], 8 if i == 0 else 3))
+    batch = types.SimpleNamespace(x=torch.randn(5, 4), ptr=torch.zeros(6, dtype=torch.long), idx=torch.zeros(0, dtype=torch.long),
+                                  etypes=torch.zeros(0, dtype=torch.long))
+    assert tuple(model(batch).shape) == (5, 3)
