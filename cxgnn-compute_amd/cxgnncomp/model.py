@@ -238,14 +238,15 @@ def get_model(config):
     """Model from a training configuration (cxgnncomp/model.py:362-399): reads
     ``dl.dataset.{feature_dim, num_classes, name}``, ``dl.sampler.train.num_layer``,
     ``train.type`` (cxg / dgl / pyg) and ``train.model.{type, hidden_dim, dropout, heads, concat,
-    num_rel}``, and ``residual`` / ``checkpoint`` where given.  The dgl / pyg graph types raise NotImplementedError."""
+    num_rel}``, and ``residual`` / ``checkpoint`` where given (false: not given); a model class is only told of
+    those that are.  The dgl / pyg graph types raise NotImplementedError."""
     dataset = config.dl.dataset
     spec = config.train.model
     kind = str(_item(spec, "type")).lower()
     graph_type = graph_type_dict[str(config.train.type).lower()]
     args = (_item(dataset, "feature_dim"), _item(spec, "hidden_dim"), _item(dataset, "num_classes"),
             config.dl.sampler.train.num_layer, _item(spec, "dropout"), graph_type, config)
-    options = dict(residual=_item(spec, "residual"), checkpoint=_item(spec, "checkpoint"))
+    options = {k: v for k, v in ((k, _item(spec, k)) for k in ("residual", "checkpoint")) if v is not None and v is not False}
     if "gat" in kind:
         return model_dict[kind](*args, **options, heads=_item(spec, "heads", 1), concat=_item(spec, "concat", False))
     if "rgcn" in kind:

@@ -31,3 +31,30 @@ def test_modules_saved_before_the_options(kind, monkeypatch):
     batch = types.SimpleNamespace(x=torch.randn(5, 4), ptr=torch.zeros(6, dtype=torch.long), idx=torch.zeros(0, dtype=torch.long),
                                   etypes=torch.zeros(0, dtype=torch.long))
     assert tuple(model(batch).shape) == (5, 3)
+
+
+def _config(**model):
+    ns = types.SimpleNamespace
+    return ns(dl=ns(dataset=ns(feature_dim=8, num_classes=4, name="x"), sampler=ns(train=ns(num_layer=3))),
+              train=ns(type="cxg", model=dict(hidden_dim=16, dropout=0.0, **model)))
+
+
+def test_configurations_without_the_options(monkeypatch):
+    """A model class of the user's own in model_dict that takes neither option, and options that are off."""
+
+    class Mine(torch.nn.Module):
+        def __init__(self, infeat, hidden, outfeat, num_layer, dropout, graph_type, config=None):
+            super().__init__()
+            self.args = (infeat, hidden, outfeat, num_layer, dropout, graph_type)
+
+    monkeypatch.setitem(cxgnncomp.model_dict, "mine", Mine)
+    assert cxgnncomp.get_model(_config(type="mine")).args == (8, 16, 4, 3, 0.0, "CSR_Layer")
+    with pytest.raises(TypeError):
+        cxgnncomp.get_model(_config(type="mine", residual="rms"))
+    for off in (None, False):
+        m = cxgnncomp.get_model(_config(type="gcn", residual=off, checkpoint=off))
+        assert m.residual is None and m.checkpoint is None and len(m.bns) == 2
+    m = cxgnncomp.get_model(_config(type="gcn", residual="layer", checkpoint="e4m3"))
+    assert m.residual == "layer" and m.checkpoint == "e4m3"
+    with pytest.raises(ValueError):
+        cxgnncomp.get_model(_config(type="gcn", residual="batch"))
