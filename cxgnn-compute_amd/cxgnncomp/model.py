@@ -15,7 +15,7 @@ Two options that upstream does not have, for deep stacks on large graphs:
     stream, r = r + gate * post(relu(layer(dropout(pre(r))))) with layer or rms norms of the rows
     (``ResidualNorm``); the first layer opens the stream, the last reads it;
   * ``checkpoint`` "int8" or "e4m3" (SAGE, GCN, GIN): the inputs of the layers' linear maps are kept
-    for the backward pass in 8 bits per value.
+    for the backward pass in 8 bits per value.  GAT and RGCN keep inputs too, in fp32, and do not take it.
 """
 import torch
 import torch.nn.functional as F
@@ -46,7 +46,7 @@ class GNN(torch.nn.Module):
         if residual not in (None, "layer", "rms"):
             raise ValueError("residual must be None, 'layer' or 'rms', got %r" % (residual, ))
         if check_format(checkpoint) is not None and not self.packs_inputs:
-            raise ValueError("%s keeps no input of a linear map that could be held in 8 bits" % type(self).__name__)
+            raise ValueError("checkpoint is taken by SAGE, GCN and GIN; the layers of %s keep what they keep as it is" % type(self).__name__)
         self.residual, self.checkpoint = residual, checkpoint
         self.in_channels = in_channels
         self.hidden_channels = hidden_channels

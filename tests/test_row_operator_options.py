@@ -58,3 +58,11 @@ def test_configurations_without_the_options(monkeypatch):
     assert m.residual == "layer" and m.checkpoint == "e4m3"
     with pytest.raises(ValueError):
         cxgnncomp.get_model(_config(type="gcn", residual="batch"))
+
+
+@pytest.mark.parametrize("kind,more", [("GAT", dict(heads=1)), ("RGCN", dict(num_rel=2))])
+def test_models_that_do_not_take_a_checkpoint_say_who_does(kind, more):
+    """(They do keep inputs of linear maps, in fp32: the refusal must not say otherwise.)"""
+    with pytest.raises(ValueError, match="taken by SAGE, GCN and GIN") as refusal:
+        getattr(cxgnncomp, kind)(4, 8, 3, 2, 0.0, "CSR_Layer", checkpoint="int8", **more)
+    assert kind in str(refusal.value)
