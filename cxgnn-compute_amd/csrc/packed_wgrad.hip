@@ -573,7 +573,8 @@ int cxg_packed_wgrad(const uint8_t* codes, const uint8_t* exps, int fmt, int64_t
   CXG_REQUIRE(value_type_ok(g_type), CXG_ERR_ARG, "unknown value type");
   CXG_REQUIRE(gw, CXG_ERR_ARG, "null gw");
   CXG_REQUIRE(seg_ptr || R == 1, CXG_ERR_ARG, "several segments need seg_ptr");
-  CXG_REQUIRE(M == 0 || (codes && exps && g && a_rows > 0 && g_rows > 0), CXG_ERR_ARG, "null codes/exps/g, or no rows");
+  const bool none = M == 0 || a_rows == 0 || g_rows == 0;       // (maps into a matrix without rows: every entry is outside)
+  CXG_REQUIRE(none || (codes && exps && g), CXG_ERR_ARG, "null codes/exps/g");
   CXG_REQUIRE(ldg >= 0, CXG_ERR_ARG, "negative row stride");
   CXG_REQUIRE(K <= kPrMaxCols && N <= kPrMaxCols && R <= 65535, CXG_ERR_UNSUPPORTED, "K, N or R too large");
   CXG_REQUIRE(((uintptr_t)codes & 15) == 0, CXG_ERR_ARG, "codes must be 16-byte aligned");
@@ -587,7 +588,7 @@ int cxg_packed_wgrad(const uint8_t* codes, const uint8_t* exps, int fmt, int64_t
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const int64_t chunks = pw_chunk_count(M, K, N, R);
   const int64_t tiles = pw_tiles(K, N);
-  const PwArgs a{codes, exps, a_rows, g, ldg, g_rows, src_idx, dst_idx, seg_ptr, M, K, N, R, packed_pitch(K), packed_groups(K),
+  const PwArgs a{codes, exps, a_rows, g, ldg, g_rows, src_idx, dst_idx, seg_ptr, none ? 0 : M, K, N, R, packed_pitch(K), packed_groups(K),
                  pw_chunk_rows(M, K, N, R), chunks, static_cast<float*>(workspace), (int64_t)K * N + (gb ? N : 0)};
   // many chunks per segment: sixteen runs of them, else four; four elements at a time where the shapes allow
   const bool many = chunks > 64 * (int64_t)R;
@@ -595,7 +596,7 @@ int cxg_packed_wgrad(const uint8_t* codes, const uint8_t* exps, int fmt, int64_t
   const int64_t sums = ceil_div(a.stride, (int64_t)(vec ? 4 : 1) * (many ? 16 : 64));           // blocks per segment
   CXG_REQUIRE(chunks * tiles < kPwMaxBlocks && sums < kPwMaxBlocks, CXG_ERR_UNSUPPORTED, "gw of %d x %d is too large for one launch",
               K, N);
-  if (M > 0) {
+  if (!none) {
     if (fmt == CXG_PACK_INT8) pw_launch_type<CXG_PACK_INT8>(a, g_type, chunks, st);
     else pw_launch_type<CXG_PACK_E4M3>(a, g_type, chunks, st);
     CXG_LAUNCH_CHECK("packed_wgrad_kernel");

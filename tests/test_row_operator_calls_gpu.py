@@ -266,3 +266,22 @@ def test_sage_layer_with_8_bits_takes_the_rows_it_takes_without(widths, num_node
     for a, b in zip(*res):
         # the same products of at most 24 values and means of about five rows, in another order
         assert float((a - b).detach().abs().max()) <= 2.0 ** -18 * float(a.detach().abs().max())
+
+
+@gpu
+@pytest.mark.parametrize("empty", ["a", "g", "both"])
+@pytest.mark.parametrize("segs", [1, 3, 20])
+def test_weight_grad_of_maps_into_matrices_without_rows(empty, segs):
+    """Every entry of such a map is outside its matrix and leaves its row out: zeros."""
+    import cxgnncomp
+    x = torch.randn(0 if empty != "g" else 50, 70, device="cuda")
+    g = torch.randn(0 if empty != "a" else 50, 33, device="cuda")
+    ids = torch.arange(50, device="cuda")
+    seg = torch.linspace(0, 50, segs + 1).long().cuda()
+    announce("packed_weight_grad of no rows %s %d" % (empty, segs))
+    p = cxgnncomp.pack_rows(x)
+    torch.full((1 << 20, ), float("nan"), device="cuda")                # (what the workspace may hold)
+    gw, gb = cxgnncomp.packed_weight_grad(p, g, seg, src_idx=ids, dst_idx=ids - (3 if empty == "both" else 0), want_sums=True)
+    assert tuple(gw.shape) == (segs, 70, 33) and tuple(gb.shape) == (segs, 33) and not gw.any() and not gb.any()
+    with pytest.raises(ValueError):                                     # no map: as many rows as there are entries are needed
+        cxgnncomp.packed_weight_grad(p, g, seg, **({"dst_idx": ids} if empty != "g" else {"src_idx": ids}))
