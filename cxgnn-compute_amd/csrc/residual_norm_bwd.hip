@@ -20,7 +20,9 @@
 // b * channel gate * (w_post, b_post) is formed once per column: a third fewer operations per value and 16
 // registers less (48 M values in rows of 8,192: bf16 181 -> 139 us, fp32 241 -> 220 us).
 // Measured: 169,343 x 256 fp32, channel gate 211 us = 4.9 TB/s; 2,449,029 x 128 bf16, element gate
-// 1.02 ms = 4.9 TB/s; the second kernel 9 us.
+// 1.02 ms = 4.9 TB/s; 187,500 x 256 fp32 beside bf16 branches 179 us = 4.8 TB/s; the second kernel 9 us.  Rows of 4,097 to
+// 8,191 columns that are no multiple of a piece spill 80 (two-byte types) to 146 registers per lane: 48 M fp32 values
+// in rows of 8,191 624 us, of 8,192 254 us.
 #include "residual_norm.hpp"
 
 namespace cxg {

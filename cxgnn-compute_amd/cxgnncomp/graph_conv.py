@@ -185,7 +185,8 @@ class MySageConv(torch.nn.Module):
 
     def __init__(self, in_channels, hidden_channels, root_weight=True, bias=True, checkpoint=None):
         """``checkpoint`` (not upstream) "int8" or "e4m3": the inputs of the layer's linear maps are kept
-        for the backward pass in 8 bits per value (``linear``)."""
+        for the backward pass in 8 bits per value (``linear``); where x is wider than the output, x and its
+        first rows apart."""
         super().__init__()
         self.checkpoint = check_format(checkpoint)
         self.in_channels = in_channels

@@ -820,8 +820,8 @@ int cxg_unpack_rows(const uint8_t* codes, const uint8_t* exps, int fmt, int64_t 
  * (bf16), two (fp16) or three (fp32) bf16 parts that add up to it exactly, accumulation is fp32 (an
  * infinity in G, or a magnitude that rounds to one in bf16, comes out as NaN or infinity).  gb (or NULL)
  * [R, N]: sums of the same rows of G, the bias gradient, from the same pass.
- * Partial sums over row chunks are added in a fixed order: results repeat bit for bit.  The workspace
- * is 256-byte aligned.
+ * Partial sums over row chunks (at most 65,536 rows) are added in a fixed order: results repeat bit for bit.
+ * The workspace is 256-byte aligned.  A gw that one launch cannot cover: CXG_ERR_UNSUPPORTED, before any launch.
  */
 size_t cxg_packed_wgrad_workspace_bytes(int64_t M, int K, int N, int R);
 int cxg_packed_wgrad(const uint8_t* codes, const uint8_t* exps, int fmt, int64_t a_rows, const void* g,
