@@ -1243,6 +1243,19 @@ std::tuple<Tensor, OptTensor> packed_wgrad(const Tensor& codes, const Tensor& ex
   return std::make_tuple(gw, gb);
 }
 
+// The sum of the rows of g [n, c] in fp32, in a fixed order (float64 rows: torch's).  Not torch's sum for the others: over
+// many blocks it clears a buffer by a memory-set node when it is captured into a graph.
+Tensor row_sum(const Tensor& g_in) {
+  if (g_in.scalar_type() == at::kDouble || g_in.size(1) == 0) return g_in.sum(0);
+  const Tensor g = g_in.to(at::kFloat).contiguous();
+  Tensor out = at::empty({g.size(1)}, g.options());
+  Tensor ws = workspace(cxg_batchnorm_workspace_bytes(g.size(0), (int)g.size(1)), g);
+  c10::DeviceGuard guard(g.device());
+  check(cxg_column_sum_f32((const float*)ptr_or_null(g), g.size(0), (int)g.size(1), g.size(1), (float*)out.data_ptr(), ws.data_ptr(),
+                           (size_t)ws.numel(), stream_of(g)));
+  return out;
+}
+
 // x W^T + bias (+ addend) with the library's product, its input kept for the weight gradient in 8 bits:
 // the compiled node of PackedLinearOP (cxgnncomp/graph_conv.py) for the shapes that the split GEMM does
 // not take, where the host's time is what counts.
@@ -1272,7 +1285,7 @@ struct PackedLinearFunction : public torch::autograd::Function<PackedLinearFunct
       out[1] = gw[0].t();                      // (autograd rounds both to the parameters' types)
       if (how[4]) out[2] = (*gb)[0];
     } else if (how[4]) {
-      out[2] = rows.sum(0);
+      out[2] = row_sum(rows);
     }
     if (how[5]) out[3] = g;
     return out;

@@ -352,7 +352,8 @@ def _weight_grad(x, g):
 
 
 def _bias_grad(g):
-    """The sum of the rows of g, in fp32 (in 64 bits for float64 rows)."""
+    """The sum of the rows of g, in fp32 in a fixed order (float64 rows: torch's sum, which over many blocks
+    does not belong into a captured graph: it clears a buffer by a memory-set node)."""
     g = g.reshape(-1, g.shape[-1])
     return g.sum(dim=0) if g.dtype == torch.float64 else _ops.column_sum(g.float().contiguous())
 
@@ -500,7 +501,7 @@ class PackedLinearOP(torch.autograd.Function):
             gw, gb = packed_weight_grad(packed, g.reshape(-1, g.shape[-1]), want_sums=True)
             gw, gb = gw[0].t(), gb[0] if ctx.needs_input_grad[2] else None      # (autograd rounds to the parameters' types)
         elif ctx.needs_input_grad[2]:
-            gb = g.reshape(-1, g.shape[-1]).sum(dim=0)
+            gb = _bias_grad(g)
         return gx, gw, gb, g if ctx.needs_input_grad[3] else None, None
 
 

@@ -285,3 +285,45 @@ def test_weight_grad_of_maps_into_matrices_without_rows(empty, segs):
     assert tuple(gw.shape) == (segs, 70, 33) and tuple(gb.shape) == (segs, 33) and not gw.any() and not gb.any()
     with pytest.raises(ValueError):                                     # no map: as many rows as there are entries are needed
         cxgnncomp.packed_weight_grad(p, g, seg, **({"dst_idx": ids} if empty != "g" else {"src_idx": ids}))
+
+
+@gpu
+@pytest.mark.parametrize("m,k,n", [(300, 90, 33), (200000, 90, 33), (200000, 128, 64), (0, 90, 33)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_bias_gradient_beside_a_frozen_weight(m, k, n, dtype):
+    """Nothing of x is kept; the sums of g's rows repeat bit for bit, eager and in a graph that is replayed between
+    eager passes."""
+    import cxgnncomp
+    torch.manual_seed(1)
+    x, w = torch.randn(m, k, device="cuda").to(dtype), torch.randn(n, k, device="cuda").to(dtype)
+    b = torch.randn(n, device="cuda").to(dtype).requires_grad_(True)
+    g = torch.randn(m, n, device="cuda").to(dtype)
+
+    def step():
+        out = cxgnncomp.linear(x, w, b, checkpoint="int8")
+        return torch.autograd.grad(out, b, g)[0]
+
+    def want():
+        v = g.double().cpu()
+        return B(v.sum(0), U * (m + 2) * 1.01 * v.abs().sum(0))
+
+    announce("linear frozen weight %d x %d x %d %s" % (m, k, n, dtype))
+    first = step()
+    check(first, want(), dtype, "bias gradient")
+    assert torch.equal(first, step())
+    if m == 0:
+        return
+    announce("linear frozen weight captured")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for _ in range(4):
+        g.mul_(1.25)
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = held.clone()
+        eager = step()
+        torch.cuda.synchronize()
+        assert torch.equal(replayed, eager)
+        check(replayed, want(), dtype, "replayed")
