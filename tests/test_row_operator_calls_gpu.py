@@ -327,3 +327,69 @@ def test_bias_gradient_beside_a_frozen_weight(m, k, n, dtype):
         torch.cuda.synchronize()
         assert torch.equal(replayed, eager)
         check(replayed, want(), dtype, "replayed")
+
+
+@gpu
+@pytest.mark.parametrize("m,k,n", [(300, 100, 47), (5000, 256, 47), (1, 64, 8)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("extra", ["bias", "addend"])
+def test_linear_on_library_products_captured_and_replayed(m, k, n, dtype, extra):
+    """The compiled node as one captured training step, replayed between eager ones with other inputs."""
+    import cxgnncomp
+    torch.manual_seed(2)
+    t = [torch.randn(s, device="cuda").to(dtype).requires_grad_(True) for s in ((m, k), (n, k), (n, ))]
+    if extra == "addend":
+        t.append(torch.randn(m, n, device="cuda").to(dtype).requires_grad_(True))
+    g = torch.randn(m, n, device="cuda").to(dtype)
+
+    def step():
+        out = cxgnncomp.linear(*t, checkpoint="e4m3")
+        return [out.detach()] + list(torch.autograd.grad(out, t, g))
+
+    announce("linear captured %d x %d x %d %s %s" % (m, k, n, dtype, extra))
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i in range(4):
+        with torch.no_grad():
+            t[0].mul_(-0.9)
+            t[1].add_(0.01)
+        g.mul_(1.125)
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [v.clone() for v in held]
+        eager = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(replayed, eager)), i
+
+
+@gpu
+def test_two_graphs_and_eager_work_keep_apart():
+    """Two captured weight gradients of different shapes, many segments in one, replayed in turns with eager work on another
+    stream: each has a workspace of its own."""
+    import cxgnncomp
+    torch.manual_seed(3)
+    cases = []
+    for m, k, n, segs in ((9000, 130, 70, 40), (4000, 300, 64, 3)):
+        p = cxgnncomp.pack_rows(torch.randn(m, k, device="cuda"))
+        cases.append((p, torch.randn(m, n, device="cuda"), torch.linspace(0, m, segs + 1).long().cuda()))
+    announce("two captured weight gradients")
+    want = [cxgnncomp.packed_weight_grad(*c, want_sums=True) for c in cases]
+    torch.cuda.synchronize()
+    graphs, held = [], []
+    for c in cases:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            held.append(cxgnncomp.packed_weight_grad(*c, want_sums=True))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        for graph in graphs:
+            graph.replay()
+        with torch.cuda.stream(side):
+            other = [cxgnncomp.packed_weight_grad(*c, want_sums=True) for c in cases]
+        torch.cuda.synchronize()
+        for got in (held, other):
+            assert all(torch.equal(a, b) for u, v in zip(got, want) for a, b in zip(u, v))
