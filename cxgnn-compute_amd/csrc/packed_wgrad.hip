@@ -96,9 +96,9 @@ __device__ __forceinline__ int64_t pw_scan(const PwArgs& a, int r0, int64_t& bef
   return n;
 }
 
-// Up to this many segments are gone through one after another (30,289 x 529 x 505 of 3 types: 64 us, 66 us by the scan;
-// 100,000 x 128 x 128 of 12: 25 us, 23 us by the scan), more of them 64 at a time (1 M x 128 x 128 of 600 types: 253 us, one after
-// another 3.6 ms).
+// Up to this many segments are gone through one after another (30,289 x 529 x 505 of 3 types: 64 us, 66 us by the
+// scan; 100,000 x 128 x 128 of 12: 25 us, 23 us by the scan), more of them 64 at a time (1 M x 128 x 128 of 600 types:
+// 253 us, one after another 3.6 ms).
 constexpr int kPwFewSegments = 8;
 
 // Chunk number -> first row and end of its rows; false past the last chunk.  Block-uniform.
@@ -119,7 +119,7 @@ __device__ __forceinline__ bool pw_locate(const PwArgs& a, int64_t chunk, int64_
       const unsigned long long here = __ballot(t >= before && t < before + n);
       found = here != 0;
       const int lane = found ? __ffsll(here) - 1 : CXG_WAVE - 1;
-      t -= __shfl(found ? before : before + n, lane, CXG_WAVE);
+      t -= uniform_i64(__shfl(found ? before : before + n, lane, CXG_WAVE));
       if (found) pw_segment(a.seg, a.M, uniform_i32(r0 + lane), b, e);
     }
   }
@@ -143,7 +143,7 @@ __device__ __forceinline__ int64_t pw_first_chunk(const PwArgs& a, int r) {
     int64_t before;
     const int64_t n = pw_scan(a, r0, before);
     const int last = r - r0 < CXG_WAVE ? r - r0 - 1 : CXG_WAVE - 1;
-    first += __shfl(before + n, last, CXG_WAVE);
+    first += uniform_i64(__shfl(before + n, last, CXG_WAVE));
   }
   return first;
 }

@@ -517,8 +517,9 @@ def _linear_product(x, weight, bias, addend):
 
 def linear(x, weight, bias=None, addend=None, checkpoint=None):
     """``F.linear(x, weight, bias)``, plus ``addend`` where given, for the conv layers; CUDA
-    tensors take LinearOP (types other than float32 its library products).  ``checkpoint`` "int8" or "e4m3": what the weight gradient needs of x is
-    kept in 8 bits per value (PackedLinearOP; CUDA tensors, float32 / bfloat16 / float16)."""
+    tensors take LinearOP (types other than float32 the library's products).  ``checkpoint`` "int8" or
+    "e4m3": what the weight gradient needs of x is kept in 8 bits per value (PackedLinearOP; CUDA tensors,
+    float32 / bfloat16 / float16)."""
     if check_format(checkpoint) is not None and x.is_cuda and torch.is_grad_enabled():     # else nothing is kept
         if addend is not None and x.dim() != 2:
             raise ValueError("an addend goes with x [N, C]")
